@@ -309,6 +309,65 @@ int launch_attn_prefill_f16kv(const float* q, const void* k16, const void* v16, 
 int launch_attn_prefill_f16kv_at(const float* q, const void* k16, const void* v16, float* out, int t, int t_kv, int q_pos0, int n_q_heads,
                                  int n_kv_heads, int head_dim, int prefix, float kq_scale, void* stream);
 
+/* ---- a KV cache in pages, and batches of sequences of different lengths.  No counterpart upstream, whose cache is one
+ * sequence (gpu-core/src/infer_ops.rs:160-189): these are the forms of launch_rope_kv_append, launch_attn_decode and
+ * launch_attn_prefill for a server that adds tokens to many sequences in one call.
+ *
+ * A batch (qmm_seq_batch, a HOST struct read during the call; the arrays it points to are device memory): the new tokens of
+ * sequence s are rows cu_q[s] .. cu_q[s+1]-1 of the packed buffers (none, one, or many); kv_len[s] is the sequence's length with
+ * them, so that row cu_q[s] + i is position kv_len[s] - (cu_q[s+1] - cu_q[s]) + i.  total_q: rows of the buffers; rows of no
+ * sequence (before cu_q[0], from cu_q[n_seqs] on) are left as they were.  max_q, max_kv: at least the largest number of new
+ * tokens and the largest kv_len (max_q chooses the kernel; kv_len beyond max_kv is cut to it).
+ * A pool (qmm_paged_kv, likewise): k_pages and v_pages (n_pages, page_size, n_kv_heads, head_dim) f16 or bf16, 16-byte aligned,
+ * pages k_page_stride / v_page_stride elements apart (multiples of 8; 0 = back to back; the two pools may be interleaved).
+ * Position t of sequence s is slot t % page_size of page page_table[s * table_stride + t / page_size]; entries past the
+ * sequence's length, and those left of every row's window, are not read, and nothing of a page but those positions counts.
+ * Arrays that point outside the buffers are not followed: a page that is not in the pool reads as zeros and takes nothing
+ * (device status 6), lengths are cut to the buffers (status 7); the outputs of such a sequence are then not meaningful.
+ *
+ * launch_rope_kv_append_paged: qkv (total_q rows, qkv_stride elements apart) of [q heads | k heads | v heads], f32, f16 or bf16.
+ *   The first rotary_dim elements (even, up to 256; 0 = none) of every q and k head are rotated as in launch_rope_kv_append
+ *   (pairs j and j + rotary_dim/2, angle position * theta^(-2j/rotary_dim), evaluated in f64); the queries go to q_out
+ *   (total_q, n_q_heads * head_dim), k and v to their slots, all in the pool's type, rounded once.  q_out distinct from qkv.
+ *   A token whose position is negative (kv_len smaller than the number of new tokens) has no slot: only its query is written.
+ * launch_attn_paged: row r of q (the pool's type) against the keys of its sequence at positions up to its own:
+ *   out[r,h] = sum_t w_t v_t / sum_t w_t, w_t = exp(kq_scale * q_r.k_t - max), over t <= position, and t > position - window
+ *   when window > 0.  A row that sees no key is 0.  out f16, bf16 or f32.  Query head h reads kv head h / (n_q_heads /
+ *   n_kv_heads), at most 64 per kv head; head_dim 32, 64, 96, 128 or 256; page_size a multiple of 8; kq_scale positive and
+ *   finite; q 16-byte aligned, q_stride a multiple of 8.  A key or value that a row does not see has no influence on it,
+ *   whatever it holds (NaN and infinities too).  scratch: qmm_attn_paged_scratch_bytes(...) bytes of caller-owned device
+ *   memory, 16-byte aligned, not shared with a call that may run at the same time; nothing in it needs clearing.
+ * launch_attn_packed: the same without a cache, for whole prompts: the keys and values are rows of the batch (kv_len and max_kv
+ *   unused; k and v in q's type, rows k_stride / v_stride elements apart, multiples of 8), so row i of a sequence sees rows 0..i
+ *   of it.
+ * Products run on the tensor cores with f32 accumulation; the probabilities are rounded to the type of v.  Bit-identical
+ * across reruns. */
+#define QMM_DT_F32 0
+#define QMM_DT_F16 1
+#define QMM_DT_BF16 2
+typedef struct {
+    const int* cu_q;    /* device, n_seqs + 1 */
+    const int* kv_len;  /* device, n_seqs */
+    int n_seqs, total_q, max_q, max_kv;
+} qmm_seq_batch;
+typedef struct {
+    const void* k_pages;
+    const void* v_pages;
+    int dtype; /* QMM_DT_F16 / BF16 */
+    int n_pages, page_size, n_kv_heads, head_dim;
+    long k_page_stride, v_page_stride;
+    const int* page_table; /* device, (n_seqs, table_stride) */
+    int table_stride;
+} qmm_paged_kv;
+int launch_rope_kv_append_paged(const void* qkv, int qkv_dtype, long qkv_stride, void* q_out, const qmm_paged_kv* kv, const qmm_seq_batch* seqs,
+                                int n_q_heads, int rotary_dim, float theta, void* stream);
+long qmm_attn_paged_scratch_bytes(int max_q, int n_q_heads, int n_kv_heads, int head_dim);
+int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, const qmm_seq_batch* seqs, void* out, int out_dtype, long out_stride,
+                      void* scratch, long scratch_bytes, int n_q_heads, int window, float kq_scale, void* stream);
+int launch_attn_packed(const void* q, const void* k, const void* v, int dtype, long q_stride, long k_stride, long v_stride,
+                       const qmm_seq_batch* seqs, void* out, int out_dtype, long out_stride, int n_q_heads, int n_kv_heads, int head_dim, int window,
+                       float kq_scale, void* stream);
+
 /* ---- quantized dense layer: y(m,n) = act( x(m,k) . w(n,k)^T + bias(n) ), x and y f32, w packed blocks of
  * `type`.  The counterpart of LayerKind::Dense in the upstream's forward pass (recipe-infer/src/forward.rs:
  * 372-431: gpu_linear_into, gpu-core/src/kernels.rs:2589-2640, then one activation launch), the place where a

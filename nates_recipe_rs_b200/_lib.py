@@ -19,6 +19,18 @@ class MatvecJob(C.Structure):
                 ("y_stride", C.c_long), ("select", C.c_void_p), ("select_stride_bytes", C.c_long), ("tp_sum", C.c_int)]
 
 
+class SeqBatch(C.Structure):
+    """qmm_seq_batch of include/qmm.h."""
+    _fields_ = [("cu_q", C.c_void_p), ("kv_len", C.c_void_p), ("n_seqs", C.c_int), ("total_q", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int)]
+
+
+class PagedKV(C.Structure):
+    """qmm_paged_kv of include/qmm.h."""
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("dtype", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("k_page_stride", C.c_long), ("v_page_stride", C.c_long),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int)]
+
+
 class GgufTensorInfo(C.Structure):
     """qmm_gguf_tensor of include/qmm_gguf.h."""
     _fields_ = [("name", C.c_char * 128), ("type", C.c_int), ("n_dims", C.c_int), ("dims", C.c_long * 4), ("file_offset", C.c_long),
@@ -82,6 +94,10 @@ SIGNATURES = {
     "launch_attn_prefill": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, C.c_float, vp]),
     "launch_attn_prefill_f16kv": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, C.c_float, vp]),
     "launch_attn_prefill_f16kv_at": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp]),
+    "launch_rope_kv_append_paged": (i32, [vp, i32, i64, vp, C.POINTER(PagedKV), C.POINTER(SeqBatch), i32, i32, C.c_float, vp]),
+    "qmm_attn_paged_scratch_bytes": (i64, [i32, i32, i32, i32]),
+    "launch_attn_paged": (i32, [vp, i64, C.POINTER(PagedKV), C.POINTER(SeqBatch), vp, i32, i64, vp, i64, i32, i32, C.c_float, vp]),
+    "launch_attn_packed": (i32, [vp, vp, vp, i32, i64, i64, i64, C.POINTER(SeqBatch), vp, i32, i64, i32, i32, i32, i32, C.c_float, vp]),
     "qmm_qdense_scratch_bytes": (i64, [i32, i32, i32]),
     "launch_qdense": (i32, [i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, C.c_float, vp]),
     "launch_moe_router_topk": (i32, [vp, vp, vp, i32, i32, i32, i32, C.c_float, C.c_float, vp, vp, vp, vp]),

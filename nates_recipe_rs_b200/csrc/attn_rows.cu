@@ -1,0 +1,593 @@
+// Attention of new tokens over a paged cache (or over packed prompts) on mma.sync: any head dimension of the library, any
+// number of rows.  The counterpart, for a batch of sequences of different lengths, of the upstream's gpu_gqa_attn_into
+// (gpu-core/src/infer_ops.rs:160-189).
+//
+//   out[r, h] = sum_t w_t V_t / sum_t w_t,  w_t = exp(kq_scale * q_r . K_t - max),  t in (pos_r - window, pos_r]
+//
+// One pass over the keys with a running maximum and sum.  The rows of a work item are (token, query head of the group) pairs
+// of ONE kv head, so a tile of keys and values fetched once serves every query head that shares it.  Decode (WM = 1, up to 16
+// rows: bound by the cache bytes): the four math warps take 16 keys each of a tile of 64 and join at the end; a fifth warp
+// keeps TMA copies of the next tiles in flight.  More rows (WM = 4, 64 rows: bound by mma.sync): a warp takes 16 rows and all
+// the keys of a tile.
+// Few items over a long axis: all (item, tile) pairs are shared out evenly over the CTAs, whatever the sequences' lengths
+// (read on the device: nothing is copied to the host).  A CTA's share begins and ends inside at most two items; those go to
+// scratch as (maximum, sum, unnormalised output) and attn_join_kernel adds them in key order, so reruns are bit identical.
+// q, k, v are f16 or bf16; the probabilities are rounded to the same type for the second product (tensor-core operands),
+// scores, maximum, sum and output stay f32.
+#include "attn_pages.cuh"
+
+namespace qmm {
+
+constexpr int AR_TILE = 64;       // keys per tile
+constexpr int AR_THREADS = 160;   // four math warps and the copying warp
+template <int HD, int WM> struct ArShape {
+    static constexpr int NCH = (HD + 63) / 64;
+    static constexpr int TILE_BYTES = NCH * AR_TILE * 128;  // one matrix
+    // two CTAs per SM up to 128 elements: about 96 KB (decode: bytes in flight) or 64 KB (many rows) of tiles each
+    static constexpr int STAGES = WM == 1 ? (HD <= 64 ? 6 : 3) : (HD <= 64 ? 4 : 2);
+    static constexpr int CTAS_PER_SM = HD <= 128 ? 2 : 1;
+    static constexpr int BUF_PITCH = HD + 4;
+    static constexpr bool Q_REGS = HD <= 128;  // the queries stay in registers (wider heads read them from shared memory)
+};
+
+struct __align__(16) ArHeader {
+    uint64_t full[8], empty[8];
+    long long scan[36];
+    float ml[4][16][2];
+    int abort_flag, nonfinite;
+};
+
+template <int HD, int WM> constexpr size_t ar_smem_bytes() {
+    using Sh = ArShape<HD, WM>;
+    return 1024 + (size_t)Sh::STAGES * 2 * Sh::TILE_BYTES + (size_t)16 * WM * (Sh::NCH * 64 + 8) * 2 + (WM == 1 ? 16 * Sh::BUF_PITCH * 4 : 0) +
+           sizeof(ArHeader);
+}
+
+// What a CTA leaves in scratch for attn_join_kernel: the item that begins in it and continues in later CTAs
+struct ArJoin {
+    int s, q0, tok_row0, n_rows;  // rows tok_row0 .. + n_rows of the sequence's (token, head of the group) list; n_rows 0: none
+    int kvh, n_parts, any_key, pad;
+};
+
+template <typename T>
+__device__ __forceinline__ void mma_16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    mma_f16_k16(d, a0, a1, a2, a3, b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma_16<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Walks the segments (item, tiles [t0, t1) of it) of this CTA; every thread of the CTA runs it and gets the same segments.
+// An item is (sequence, kv head, block of R rows); all items of a sequence count the tiles of the whole sequence, at least one.
+template <int R>
+struct ArWalker {
+    const AttnParams& p;
+    long g, g1;        // this CTA's share of all tiles: [g, g1)
+    int s, item, within;
+    SeqInfo si;
+    int tl, nt, nrb;   // of sequence s: first tile, tiles per item, row blocks
+    // of the current segment
+    int t0, t1, kvh, rb;
+    bool begins, ends;
+
+    __device__ __forceinline__ void load_seq() {
+        si = seq_info(p, s);
+        const KeyRange kr = key_range(p, si, 0, si.q_len);
+        tl = kr.a / AR_TILE;
+        nt = max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - tl);
+        nrb = (si.q_len * p.group + R - 1) / R;
+    }
+    __device__ static __forceinline__ long tiles_of(const AttnParams& p, int s) {
+        const SeqInfo si = seq_info(p, s);
+        const KeyRange kr = key_range(p, si, 0, si.q_len);
+        return (long)((si.q_len * p.group + R - 1) / R) * p.nkv * max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - kr.a / AR_TILE);
+    }
+    __device__ __forceinline__ bool next() {
+        if (g >= g1) return false;
+        while (item >= nrb * p.nkv) {  // (sequences without rows have no items)
+            if (++s >= p.n_seqs) return false;
+            item = within = 0;
+            load_seq();
+        }
+        const int n = (int)min(g1 - g, (long)(nt - within));
+        kvh = item / nrb, rb = item - kvh * nrb;
+        t0 = tl + within, t1 = t0 + n;
+        begins = within == 0, ends = within + n == nt;
+        g += n, within += n;
+        if (within == nt) within = 0, ++item;
+        return true;
+    }
+};
+// First tile of CTA c of n when `total` tiles are shared evenly
+__device__ __forceinline__ long ar_share(long total, int c, int n) { return total * c / n; }
+constexpr int AR_MIN_TILES = 2;  // fewer tiles than this per CTA: fewer CTAs (a share of one tile costs more in joining than it saves)
+__device__ __forceinline__ int ar_ctas(long total, int grid) { return (int)max(1l, min((long)grid, total / AR_MIN_TILES)); }
+
+template <int HD, int R> struct ArScratch {  // layout of the scratch: joins, then per CTA two slots of (m, l) and outputs
+    __host__ __device__ static size_t join_floats(int ctas) { return (size_t)ctas * (sizeof(ArJoin) / 4); }
+    __host__ __device__ static size_t floats(int ctas) { return join_floats(ctas) + (size_t)ctas * 2 * R * (HD + 2); }
+    __device__ static float* ml(float* base, int ctas, int slot) { return base + join_floats(ctas) + (size_t)slot * R * 2; }
+    __device__ static float* o(float* base, int ctas, int slot) { return base + join_floats(ctas) + (size_t)ctas * 2 * R * 2 + (size_t)slot * R * HD; }
+};
+
+template <typename T, int HD, int WM>
+__global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) attn_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                                                               const __grid_constant__ AttnParams p) {
+    using Sh = ArShape<HD, WM>;
+    constexpr int R = 16 * WM, WN = 4 / WM, KW = AR_TILE / WN;  // rows of an item, warps along the keys, keys per warp and tile
+    constexpr int NT = KW / 8, QPITCH = Sh::NCH * 64 + 8;
+    extern __shared__ __align__(1024) uint8_t ar_raw[];
+    uint8_t* sm = ar_raw + ((1024u - (smem_u32(ar_raw) & 1023u)) & 1023u);
+    const uint32_t ring = smem_u32(sm);
+    T* qs = reinterpret_cast<T*>(sm + (size_t)Sh::STAGES * 2 * Sh::TILE_BYTES);
+    float* buf = reinterpret_cast<float*>(qs + R * QPITCH);  // (WM == 1) one 16 x HD output while the warps join
+    ArHeader* hdr = reinterpret_cast<ArHeader*>(reinterpret_cast<uint8_t*>(buf) + (WM == 1 ? 16 * Sh::BUF_PITCH * 4 : 0));
+    volatile int* cta_abort = &hdr->abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < Sh::STAGES; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), 4);
+        hdr->abort_flag = 0, hdr->nonfinite = 0;
+        mbar_fence_init();
+    }
+    pdl_wait_prior_grids();
+    pdl_release_dependents();
+
+    ArWalker<R> w{p};
+    int n_ctas = 1;
+    long total = 0;  // tiles of the whole batch (shared evenly)
+    if (p.stream_k) {
+        // all tiles, then the sequence this CTA's share starts in
+        long before = 0;
+        find_item(p.n_seqs, 1l << 62, [&](int s) { return ArWalker<R>::tiles_of(p, s); }, total, hdr->scan);
+        n_ctas = ar_ctas(total, gridDim.x);
+        ArJoin* join = reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x;
+        if (tid == 0) join->n_rows = 0;
+        if ((int)blockIdx.x >= n_ctas) return;
+        w.g = ar_share(total, blockIdx.x, n_ctas), w.g1 = ar_share(total, blockIdx.x + 1, n_ctas);
+        w.s = find_item(p.n_seqs, w.g, [&](int s) { return ArWalker<R>::tiles_of(p, s); }, before, hdr->scan);
+        if (w.s < 0) return;  // (no rows at all)
+        w.load_seq();
+        w.item = (int)((w.g - before) / w.nt), w.within = (int)((w.g - before) % w.nt);
+    } else {
+        // one item per CTA: block row blockIdx.y of all row blocks (a sequence's last, longest, first), kv head blockIdx.x
+        long before = 0;
+        w.s = find_item(p.n_seqs, blockIdx.y, [&](int s) { return ((long)seq_info(p, s).q_len * p.group + R - 1) / R; }, before, hdr->scan);
+        if (w.s < 0) return;
+        w.load_seq();
+        w.g = 0, w.g1 = w.nt, w.within = 0;
+        w.item = blockIdx.x * w.nrb + (w.nrb - 1 - (int)(blockIdx.y - before));
+    }
+    __syncthreads();
+    int it = 0;  // tiles so far, over all segments: stage it % STAGES
+
+    auto give_up = [&](int code) {
+        if (!*cta_abort) {
+            raise_status(code);
+            *cta_abort = 1;
+        }
+    };
+    // the tokens of a row block, and the tiles of a segment that hold keys of its rows
+    auto block_range = [&](int& tok0, int& n_rows, KeyRange& kr, int& t0, int& t1) {
+        const int r0 = w.rb * R;
+        n_rows = min(R, w.si.q_len * p.group - r0);
+        tok0 = r0 / p.group;
+        kr = key_range(p, w.si, tok0, (r0 + n_rows - 1) / p.group + 1);
+        t0 = max(w.t0, kr.a / AR_TILE), t1 = min(w.t1, (kr.b + AR_TILE - 1) / AR_TILE);
+    };
+
+    if (warp == 4) {
+        // ------------------------------------------------------------ copies
+        while (!*cta_abort && w.next()) {
+            int tok0, n_rows, t0, t1;
+            KeyRange kr;
+            block_range(tok0, n_rows, kr, t0, t1);
+            int first, count, pages = 0;
+            if (t0 < t1) {
+                tile_boxes<AR_TILE>(p, t0, kr.a, kr.b, first, count);
+                pages = page_of_boxes<AR_TILE>(p, w.s, t0, first, count);
+            }
+            for (int t = t0; t < t1; ++t, ++it) {
+                const int st = it % Sh::STAGES;
+                int nfirst = 0, ncount = 0, npages = 0;
+                if (t + 1 < t1) {  // the next tile's pages are looked up before this tile's turn comes
+                    tile_boxes<AR_TILE>(p, t + 1, kr.a, kr.b, nfirst, ncount);
+                    npages = page_of_boxes<AR_TILE>(p, w.s, t + 1, nfirst, ncount);
+                }
+                if (it >= Sh::STAGES && !mbar_wait_bounded(smem_u32(&hdr->empty[st]), ((it / Sh::STAGES) - 1) & 1, cta_abort)) {
+                    if (lane == 0) give_up(DEV_TIMEOUT_EMPTY);
+                    break;
+                }
+                const uint32_t bar = smem_u32(&hdr->full[st]), dst = ring + (uint32_t)st * 2 * Sh::TILE_BYTES;
+                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)count * 2 * Sh::NCH * p.box_rows * 128);
+                __syncwarp();
+                load_tile<AR_TILE, Sh::NCH>(p, &kmap, dst, bar, t, first, count, pages, w.si.q0, w.kvh);
+                load_tile<AR_TILE, Sh::NCH>(p, &vmap, dst + Sh::TILE_BYTES, bar, t, first, count, pages, w.si.q0, w.kvh);
+                first = nfirst, count = ncount, pages = npages;
+            }
+        }
+        // copies in flight land before the CTA ends (on every path: after a normal run the consumers have seen them all)
+        if (*cta_abort) {
+            for (int i = max(0, it - Sh::STAGES); i < it; ++i) {
+                const long long c0 = clock64();
+                while (!mbar_try_wait(smem_u32(&hdr->full[i % Sh::STAGES]), (i / Sh::STAGES) & 1))
+                    if (clock64() - c0 > WAIT_LIMIT_CYCLES) {
+                        raise_status(DEV_TIMEOUT_DRAIN);
+                        break;
+                    }
+            }
+        }
+        return;
+    }
+
+    // ---------------------------------------------------------------- math warps
+    const int qr = lane >> 2, pq = lane & 3;
+    const int row_w = WM == 1 ? 0 : 16 * warp, key_w = WM == 1 ? KW * warp : 0;  // this warp's rows and keys of a tile
+    while (w.next()) {
+        int tok0, n_rows, t0, t1;
+        KeyRange kr;
+        block_range(tok0, n_rows, kr, t0, t1);
+        const int r0 = w.rb * R;
+        // queries to shared memory (elements past HD and rows past the block: zeros), then to registers as A fragments
+        math_sync();  // the fragments and the buffer of the segment before have been read
+        for (int i = tid; i < R * Sh::NCH * 8; i += 128) {
+            const int r = i / (Sh::NCH * 8), c = (i - r * (Sh::NCH * 8)) * 8;
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (r < n_rows && c < HD) {
+                const int tok = (r0 + r) / p.group, h = w.kvh * p.group + (r0 + r) % p.group;
+                x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (size_t)(w.si.q0 + tok) * p.q_stride + (size_t)h * HD + c);
+            }
+            *reinterpret_cast<uint4*>(qs + r * QPITCH + c) = x;
+        }
+        math_sync();
+        // this thread's two rows: the keys [lo, hi) they see
+        int lo[2], hi[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = row_w + qr + 8 * e;
+            const int pos = w.si.kv - w.si.q_len + (r0 + r) / p.group;
+            hi[e] = r < n_rows ? max(pos + 1, 0) : 0;
+            lo[e] = p.window ? max(0, pos - p.window + 1) : 0;
+        }
+        uint32_t qf[Sh::Q_REGS ? HD / 16 : 1][4];
+        const uint32_t qa = smem_u32(qs + (row_w + (lane & 15)) * QPITCH + (lane >> 4) * 8);
+        if constexpr (Sh::Q_REGS) {
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) ldsm_x4(qf[kk], qa + kk * 32);
+        }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float o[HD / 8][4];
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+
+        for (int t = t0; t < t1; ++t, ++it) {
+            const int st = it % Sh::STAGES;
+            if (!mbar_wait_bounded(smem_u32(&hdr->full[st]), (it / Sh::STAGES) & 1, cta_abort)) {
+                if (lane == 0) give_up(DEV_TIMEOUT_FULL);  // (on to the end all the same: the warps meet at barriers)
+            }
+            const uint32_t ks = ring + (uint32_t)st * 2 * Sh::TILE_BYTES, vs = ks + Sh::TILE_BYTES;
+            const int k0 = t * AR_TILE;
+            const bool masked = k0 < kr.a2 || k0 + AR_TILE > kr.b2;  // some row does not see some key of the tile
+            if (masked) {
+                // values that no row sees become zeros; where some row does not see a key, a value that is not finite
+                // does too, and the rows are computed again without the tensor cores (attn_row_exact)
+                uint8_t* vp = sm + (size_t)st * 2 * Sh::TILE_BYTES + Sh::TILE_BYTES;
+                bool odd = false;
+                for (int i = tid; i < Sh::NCH * AR_TILE * 8; i += 128) {
+                    const int key = k0 + ((i >> 3) % AR_TILE);
+                    if (key >= kr.a2 && key < kr.b2) continue;
+                    uint4* x = reinterpret_cast<uint4*>(vp) + i;
+                    if (key < kr.a || key >= kr.b) {
+                        *x = make_uint4(0u, 0u, 0u, 0u);
+                    } else {
+                        const uint4 y = *x;
+                        if (has_nonfinite<T>(y.x) || has_nonfinite<T>(y.y) || has_nonfinite<T>(y.z) || has_nonfinite<T>(y.w)) {
+                            *x = make_uint4(0u, 0u, 0u, 0u);
+                            odd = true;
+                        }
+                    }
+                }
+                if (odd) hdr->nonfinite = 1;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage is refilled by a copy
+                math_sync();
+            }
+            // scores: 16 rows x KW keys
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                uint32_t(&a)[4] = qf[Sh::Q_REGS ? kk : 0];
+                if constexpr (!Sh::Q_REGS) ldsm_x4(a, qa + kk * 32);
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    const int row = key_w + 8 * n + (lane & 7) + ((lane >> 4) & 1) * 8, c = kk * 16 + ((lane >> 3) & 1) * 8;
+                    uint32_t b[4];
+                    ldsm_x4(b, ks + (uint32_t)((c >> 6) * AR_TILE + row) * 128u + ((((uint32_t)(c & 63) >> 3) ^ (row & 7)) << 4));
+                    mma_16<T>(sc[n], a[0], a[1], a[2], a[3], b[0], b[1]);
+                    mma_16<T>(sc[n + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = k0 + key_w + 8 * n + 2 * pq + (e & 1);
+                        if (key < lo[e >> 1] || key >= hi[e >> 1]) sc[n][e] = -INFINITY;
+                    }
+            }
+            // running softmax (m in raw scores; kq_scale > 0)
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mx[0] = fmaxf(mx[0], fmaxf(sc[n][0], sc[n][1])), mx[1] = fmaxf(mx[1], fmaxf(sc[n][2], sc[n][3]));
+            bool grew = false;
+            float mu[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+                grew |= mx[e] > m[e];
+            }
+            if (__any_sync(0xffffffffu, grew)) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mn = fmaxf(m[e], mx[e]);
+                    f[e] = mn == -INFINITY ? 1.f : fast_exp2((m[e] - mn) * p.scale_log2);
+                    m[e] = mn, l[e] *= f[e];
+                }
+#pragma unroll
+                for (int n = 0; n < HD / 8; ++n) o[n][0] *= f[0], o[n][1] *= f[0], o[n][2] *= f[1], o[n][3] *= f[1];
+            }
+            mu[0] = m[0] == -INFINITY ? 0.f : m[0], mu[1] = m[1] == -INFINITY ? 0.f : m[1];
+            uint32_t pa[NT / 2][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float e0 = fast_exp2((sc[n][0] - mu[0]) * p.scale_log2), e1 = fast_exp2((sc[n][1] - mu[0]) * p.scale_log2);
+                const float e2 = fast_exp2((sc[n][2] - mu[1]) * p.scale_log2), e3 = fast_exp2((sc[n][3] - mu[1]) * p.scale_log2);
+                l[0] += e0 + e1, l[1] += e2 + e3;
+                pa[n >> 1][(n & 1) * 2] = pack2<T>(e0, e1);
+                pa[n >> 1][(n & 1) * 2 + 1] = pack2<T>(e2, e3);
+            }
+            // outputs: P (16 x KW) . V (KW x HD)
+#pragma unroll
+            for (int j = 0; j < NT / 2; ++j) {
+                const int row = key_w + 16 * j + (lane & 15);
+#pragma unroll
+                for (int n = 0; n < HD / 8; n += 2) {
+                    const int c = 8 * n + ((lane >> 4) & 1) * 8;
+                    uint32_t b[4];
+                    ldsm_x4_t(b, vs + (uint32_t)((c >> 6) * AR_TILE + row) * 128u + ((((uint32_t)(c & 63) >> 3) ^ (row & 7)) << 4));
+                    mma_16<T>(o[n], pa[j][0], pa[j][1], pa[j][2], pa[j][3], b[0], b[1]);
+                    mma_16<T>(o[n + 1], pa[j][0], pa[j][1], pa[j][2], pa[j][3], b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&hdr->empty[st]));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        }
+
+        // where the segment's result goes: the output rows, or a slot of scratch (0: continues an item, 1: begins one)
+        const bool whole = w.begins && w.ends;
+        const int slot = 2 * (int)blockIdx.x + (w.begins ? 1 : 0);
+        float* sml = whole ? nullptr : ArScratch<HD, R>::ml(p.scratch, gridDim.x, slot);
+        float* so = whole ? nullptr : ArScratch<HD, R>::o(p.scratch, gridDim.x, slot);
+        auto out_elem = [&](int r) {  // element index of row r's first output
+            const int tok = (r0 + r) / p.group, h = w.kvh * p.group + (r0 + r) % p.group;
+            return (size_t)(w.si.q0 + tok) * p.out_stride + (size_t)h * HD;
+        };
+        auto row_sees = [&](int r) {  // row r has keys at all (else its output is 0)
+            return w.si.kv - w.si.q_len + (r0 + r) / p.group >= 0;
+        };
+        math_sync();  // every warp's verdict on the values
+        const bool exact = hdr->nonfinite != 0;
+        math_sync();
+        if (exact) {
+            if (tid == 0) hdr->nonfinite = 0;
+            for (int r = warp; r < n_rows; r += 4) {
+                const int tok = (r0 + r) / p.group, pos = w.si.kv - w.si.q_len + tok;
+                float em, el, eo[HD / 32];
+                attn_row_exact<T, HD>(p, w.s, w.si.q0, tok, w.kvh * p.group + (r0 + r) % p.group, w.kvh,
+                                      max(w.t0 * AR_TILE, p.window ? max(0, pos - p.window + 1) : 0), min(w.t1 * AR_TILE, pos + 1), em, el, eo);
+                const float inv = row_sees(r) ? 1.f / el : 0.f;
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) {
+                    if (whole) store_out1(p.out, p.out_dtype, out_elem(r) + lane + 32 * j, row_sees(r) ? eo[j] * inv : 0.f);
+                    else so[(size_t)r * HD + lane + 32 * j] = eo[j];
+                }
+                if (!whole && lane == 0) sml[2 * r] = em, sml[2 * r + 1] = el;
+            }
+        } else if constexpr (WM == 1) {
+            // the four warps' parts, added in warp order through one buffer
+            if (pq == 0)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) hdr->ml[warp][qr + 8 * e][0] = m[e], hdr->ml[warp][qr + 8 * e][1] = l[e];
+            math_sync();
+            float f[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = qr + 8 * e;
+                const float mm = fmaxf(fmaxf(hdr->ml[0][r][0], hdr->ml[1][r][0]), fmaxf(hdr->ml[2][r][0], hdr->ml[3][r][0]));
+                f[e] = m[e] == -INFINITY ? 0.f : fast_exp2((m[e] - mm) * p.scale_log2);
+            }
+            for (int u = 0; u < 4; ++u) {
+                if (warp == u) {
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float2* d = reinterpret_cast<float2*>(buf + (qr + 8 * e) * Sh::BUF_PITCH + 8 * n + 2 * pq);
+                            float2 x = u == 0 ? make_float2(0.f, 0.f) : *d;
+                            // (a warp without keys has zeros, which a factor of 0 keeps; one with a NaN keeps that too)
+                            x.x += o[n][2 * e] * f[e], x.y += o[n][2 * e + 1] * f[e];
+                            *d = x;
+                        }
+                }
+                math_sync();
+            }
+            for (int i = tid; i < n_rows * (HD / 2); i += 128) {
+                const int r = i / (HD / 2), c = (i - r * (HD / 2)) * 2;
+                float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) mm = fmaxf(mm, hdr->ml[u][r][0]);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) ll += hdr->ml[u][r][0] == -INFINITY ? hdr->ml[u][r][1] : hdr->ml[u][r][1] * fast_exp2((hdr->ml[u][r][0] - mm) * p.scale_log2);
+                const float2 x = *reinterpret_cast<const float2*>(buf + r * Sh::BUF_PITCH + c);
+                if (whole) {
+                    const float inv = row_sees(r) ? 1.f / ll : 0.f;
+                    store_out2(p.out, p.out_dtype, out_elem(r) + c, row_sees(r) ? x.x * inv : 0.f, row_sees(r) ? x.y * inv : 0.f);
+                } else {
+                    *reinterpret_cast<float2*>(so + (size_t)r * HD + c) = x;
+                    if (c == 0) sml[2 * r] = mm, sml[2 * r + 1] = ll;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = row_w + qr + 8 * e;
+                if (r < n_rows) {
+                    const bool sees = row_sees(r);
+                    const float inv = sees ? 1.f / l[e] : 0.f;
+                    const size_t oe = out_elem(r);
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n) {
+                        if (whole) store_out2(p.out, p.out_dtype, oe + 8 * n + 2 * pq, sees ? o[n][2 * e] * inv : 0.f, sees ? o[n][2 * e + 1] * inv : 0.f);
+                        else *reinterpret_cast<float2*>(so + (size_t)r * HD + 8 * n + 2 * pq) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
+                    }
+                    if (!whole && pq == 0) sml[2 * r] = m[e], sml[2 * r + 1] = l[e];
+                }
+            }
+        }
+        if (w.begins && !w.ends && tid == 0) {
+            // this item goes on in the next CTAs: how many of them
+            ArJoin j;
+            j.s = w.s, j.q0 = w.si.q0, j.tok_row0 = r0, j.n_rows = n_rows, j.kvh = w.kvh;
+            j.any_key = w.si.kv - w.si.q_len;  // position of token 0
+            const long item_end = w.g1 + (w.nt - (w.t1 - w.tl));  // (a segment that does not end its item ends the share)
+            int c = blockIdx.x + 1;
+            while (ar_share(total, c + 1, n_ctas) < item_end) ++c;
+            j.n_parts = c - (int)blockIdx.x + 1, j.pad = 0;
+            reinterpret_cast<ArJoin*>(p.scratch)[blockIdx.x] = j;
+        }
+    }
+}
+
+// Adds the parts of the items that several CTAs share, in key order.  A warp per row.
+template <int HD, int R>
+__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnParams p, int ctas) {
+    pdl_wait_prior_grids();
+    const ArJoin j = reinterpret_cast<const ArJoin*>(p.scratch)[blockIdx.x];
+    const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= j.n_rows) return;
+    const int c0 = blockIdx.x;
+    auto slot_of = [&](int i) { return 2 * (c0 + i) + (i == 0 ? 1 : 0); };
+    float mm = -INFINITY;
+    for (int i = lane; i < j.n_parts; i += 32) mm = fmaxf(mm, ArScratch<HD, R>::ml(p.scratch, ctas, slot_of(i))[2 * r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    const float mu = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f, acc[HD / 32];
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) acc[e] = 0.f;
+    for (int i0 = 0; i0 < j.n_parts; i0 += 32) {
+        float f = 0.f, lp = 0.f;
+        if (i0 + lane < j.n_parts) {
+            const float* ml = ArScratch<HD, R>::ml(p.scratch, ctas, slot_of(i0 + lane)) + 2 * r;
+            f = fast_exp2((ml[0] - mu) * p.scale_log2);
+            // (a part without keys: maximum -inf, sum 0; its factor of 0 keeps both)
+            lp = ml[1] * f;
+            if (ml[1] != ml[1]) lp = ml[1];
+        }
+        const int n = min(32, j.n_parts - i0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float fi = __shfl_sync(0xffffffffu, f, i);
+            ll += __shfl_sync(0xffffffffu, lp, i);
+            const float* o = ArScratch<HD, R>::o(p.scratch, ctas, slot_of(i0 + i)) + (size_t)r * HD;
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) acc[e] += o[lane + 32 * e] * fi;
+        }
+    }
+    const int tok = (j.tok_row0 + r) / p.group, h = j.kvh * p.group + (j.tok_row0 + r) % p.group;
+    const bool sees = j.any_key + tok >= 0;
+    const float inv = 1.f / ll;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e)
+        store_out1(p.out, p.out_dtype, (size_t)(j.q0 + tok) * p.out_stride + (size_t)h * HD + lane + 32 * e, sees ? acc[e] * inv : 0.f);
+}
+
+// ---- host side ----
+template <typename T, int HD, int WM>
+static int attn_rows_inst(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+    constexpr int R = 16 * WM;
+    constexpr size_t smem = ar_smem_bytes<HD, WM>();
+    static std::mutex mu;
+    static bool configured[64] = {};
+    int dev = 0;
+    QMM_CUDA_TRY(cudaGetDevice(&dev));
+    {
+        std::lock_guard<std::mutex> g(mu);
+        if (dev < 0 || dev >= 64 || !configured[dev]) {
+            QMM_CUDA_TRY(cudaFuncSetAttribute(attn_rows_kernel<T, HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            if (dev >= 0 && dev < 64) configured[dev] = true;
+        }
+    }
+    const int ctas = sm_count() * ArShape<HD, WM>::CTAS_PER_SM;
+    const long blocks = (long)p.total_q * p.group / R + p.n_seqs;  // at least as many as row blocks there are
+    dim3 grid = p.stream_k ? dim3(ctas) : dim3(p.nkv, (unsigned)blocks);
+    if (!p.stream_k && blocks > 65535) return QMM_ERR_UNSUPPORTED;
+    if (int st = launch_overlapped(attn_rows_kernel<T, HD, WM>, grid, dim3(AR_THREADS), smem, s, km, vm, p)) return st;
+    if (p.stream_k) return launch_overlapped(attn_join_kernel<HD, R>, dim3(ctas, R / 4), dim3(128), 0, s, p, ctas);
+    return QMM_OK;
+}
+
+template <int HD> static long ar_scratch_floats_hd(bool narrow) {
+    return narrow ? (long)ArScratch<HD, 16>::floats(sm_count() * ArShape<HD, 1>::CTAS_PER_SM) : (long)ArScratch<HD, 64>::floats(sm_count() * ArShape<HD, 4>::CTAS_PER_SM);
+}
+static long attn_rows_scratch_bytes(int hd, bool narrow) {
+    switch (hd) {
+    case 32: return 4 * ar_scratch_floats_hd<32>(narrow);
+    case 64: return 4 * ar_scratch_floats_hd<64>(narrow);
+    case 96: return 4 * ar_scratch_floats_hd<96>(narrow);
+    case 128: return 4 * ar_scratch_floats_hd<128>(narrow);
+    case 256: return 4 * ar_scratch_floats_hd<256>(narrow);
+    }
+    return QMM_ERR_UNSUPPORTED;
+}
+// CTAs that run at once: fewer items than this leave the GPU partly idle unless the items are shared
+static int attn_rows_slots(int hd) { return sm_count() * (hd <= 128 ? 2 : 1); }
+
+int attn_rows_launch(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, int dtype, int hd, bool narrow, cudaStream_t s) {
+#define QMM_AR_CASE(HD_)                                                                                                                       \
+    case HD_:                                                                                                                                  \
+        if (dtype == QMM_DT_F16) return narrow ? attn_rows_inst<__half, HD_, 1>(p, km, vm, s) : attn_rows_inst<__half, HD_, 4>(p, km, vm, s);  \
+        return narrow ? attn_rows_inst<__nv_bfloat16, HD_, 1>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, HD_, 4>(p, km, vm, s)
+    switch (hd) {
+        QMM_AR_CASE(32);
+        QMM_AR_CASE(64);
+        QMM_AR_CASE(96);
+        QMM_AR_CASE(128);
+        QMM_AR_CASE(256);
+    }
+#undef QMM_AR_CASE
+    return QMM_ERR_UNSUPPORTED;
+}
+
+}  // namespace qmm

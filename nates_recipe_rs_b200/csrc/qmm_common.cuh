@@ -24,6 +24,8 @@ enum DeviceStatus : int {
     DEV_TIMEOUT_DRAIN = 3,  // producer gave up waiting for its own copies at exit
     DEV_TIMEOUT_MMA = 4,    // GEMM: gave up waiting for tensor-core completion
     DEV_TIMEOUT_PEER = 5,   // allreduce: gave up waiting for a peer's flag
+    DEV_BAD_PAGE = 6,       // paged cache: a page table entry in use is not a page of the pool
+    DEV_BAD_LENGTH = 7,     // paged cache: cu_q or kv_len goes outside the buffers
 };
 // (libqmm is built as ONE translation unit, so this is a single word per device.)
 static __device__ int g_device_status = 0;
