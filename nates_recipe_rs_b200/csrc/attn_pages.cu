@@ -63,8 +63,21 @@ static int check_out(const void* out, int dtype, long stride, int nqh, int hd) {
 }
 static bool bad_scale(float s) { return !(s > 0.f) || std::isinf(s); }
 
-// Up to 16 (token, query head of the group) rows per sequence and kv head: the decode form
-static bool narrow_rows(long max_q, int group) { return max_q * group <= 16; }
+// The three forms: up to 16 (token, query head of the group) rows per sequence and kv head (decode: bound by the cache), more
+// rows on tcgen05, more rows on mma.sync for the head dimensions that the tcgen05 kernel does not have.
+enum AttnForm { ATTN_NARROW, ATTN_TILES, ATTN_WIDE };
+static AttnForm attn_form(long max_q, int group, int hd) {
+    return max_q * group <= 16 ? ATTN_NARROW : attn_tiles_fits(hd) ? ATTN_TILES : ATTN_WIDE;
+}
+static int attn_run_form(AttnForm form, AttnParams& p, int dtype, int hd, long rows, long n_pages, cudaStream_t s) {
+    const int tile = form == ATTN_TILES ? AT_TILE : AR_TILE;
+    p.box_rows = p.table ? gcd_int(p.page_size, tile) : tile;
+    CUtensorMap km, vm;
+    if (int st = kv_tensor_map(&km, p.k, dtype, hd, p.nkv, rows, n_pages, p.k_row, p.k_page, p.box_rows)) return st;
+    if (int st = kv_tensor_map(&vm, p.v, dtype, hd, p.nkv, rows, n_pages, p.v_row, p.v_page, p.box_rows)) return st;
+    if (form == ATTN_TILES) return attn_tiles_launch(p, km, vm, dtype, hd, s);
+    return attn_rows_launch(p, km, vm, dtype, hd, form == ATTN_NARROW, s);
+}
 
 }  // namespace qmm
 
@@ -111,7 +124,8 @@ int launch_rope_kv_append_paged(const void* qkv, int qkv_dtype, long qkv_stride,
 long qmm_attn_paged_scratch_bytes(int max_q, int n_q_heads, int n_kv_heads, int head_dim) {
     if (max_q < 0) return QMM_ERR_SHAPE;
     if (int st = check_heads(n_q_heads, n_kv_heads, head_dim)) return st;
-    return attn_rows_scratch_bytes(head_dim, narrow_rows(max_q, n_q_heads / n_kv_heads));
+    const AttnForm form = attn_form(max_q, n_q_heads / n_kv_heads, head_dim);
+    return form == ATTN_TILES ? attn_tiles_scratch_bytes(head_dim) : attn_rows_scratch_bytes(head_dim, form == ATTN_NARROW);
 }
 
 int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, const qmm_seq_batch* seqs, void* out, int out_dtype, long out_stride,
@@ -126,8 +140,7 @@ int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, cons
     if (q_stride < (long)n_q_heads * hd || window < 0 || bad_scale(kq_scale) || out == q) return QMM_ERR_SHAPE;
     if (kv->page_size % 8) return QMM_ERR_UNSUPPORTED;
     if (misaligned(q, 16) || q_stride % 8 || misaligned(scratch, 16)) return QMM_ERR_ALIGN;
-    const bool narrow = narrow_rows(seqs->max_q, n_q_heads / nkv);
-    if (scratch_bytes < attn_rows_scratch_bytes(hd, narrow)) return QMM_ERR_SCRATCH;
+    if (scratch_bytes < qmm_attn_paged_scratch_bytes(seqs->max_q, n_q_heads, nkv, hd)) return QMM_ERR_SCRATCH;
     if (seqs->total_q == 0) return QMM_OK;
     p.q = q, p.k = kv->k_pages, p.v = kv->v_pages, p.out = out;
     p.table = kv->page_table, p.cu_q = seqs->cu_q, p.kv_len = seqs->kv_len, p.scratch = static_cast<float*>(scratch);
@@ -136,13 +149,11 @@ int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, cons
     p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = seqs->max_kv;
     p.nqh = n_q_heads, p.nkv = nkv, p.group = n_q_heads / nkv, p.window = window, p.out_dtype = out_dtype;
     p.scale_log2 = kq_scale * 1.4426950408889634f;
-    p.box_rows = gcd_int(p.page_size, AR_TILE);
-    // decode, and more rows where their blocks would not fill the GPU: the tiles are shared evenly
-    p.stream_k = narrow || ((long)p.total_q * p.group / 64 + 1) * nkv < 2l * attn_rows_slots(hd);
-    CUtensorMap km, vm;
-    if (int st = kv_tensor_map(&km, p.k, kv->dtype, hd, nkv, p.page_size, p.n_pages, p.k_row, p.k_page, p.box_rows)) return st;
-    if (int st = kv_tensor_map(&vm, p.v, kv->dtype, hd, nkv, p.page_size, p.n_pages, p.v_row, p.v_page, p.box_rows)) return st;
-    return attn_rows_launch(p, km, vm, kv->dtype, hd, narrow, as_stream(stream));
+    // decode, and more rows where their items would not fill the GPU several times over: the tiles are shared evenly
+    const AttnForm form = attn_form(seqs->max_q, p.group, hd);
+    const long items = ((long)p.total_q * p.group / (form == ATTN_TILES ? AT_MAX_ROWS : 64) + 1) * nkv;
+    p.stream_k = form == ATTN_NARROW || items < 4l * sm_count();
+    return attn_run_form(form, p, kv->dtype, hd, p.page_size, p.n_pages, as_stream(stream));
 }
 
 int launch_attn_packed(const void* q, const void* k, const void* v, int dtype, long q_stride, long k_stride, long v_stride,
@@ -166,11 +177,8 @@ int launch_attn_packed(const void* q, const void* k, const void* v, int dtype, l
     p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = seqs->max_q;
     p.nqh = n_q_heads, p.nkv = nkv, p.group = n_q_heads / nkv, p.window = window, p.out_dtype = out_dtype;
     p.scale_log2 = kq_scale * 1.4426950408889634f;
-    p.box_rows = AR_TILE;
-    CUtensorMap km, vm;
-    if (int st = kv_tensor_map(&km, k, dtype, hd, nkv, p.total_q, 1, k_stride, (long)p.total_q * k_stride, p.box_rows)) return st;
-    if (int st = kv_tensor_map(&vm, v, dtype, hd, nkv, p.total_q, 1, v_stride, (long)p.total_q * v_stride, p.box_rows)) return st;
-    return attn_rows_launch(p, km, vm, dtype, hd, false, as_stream(stream));
+    p.k_page = (long)p.total_q * k_stride, p.v_page = (long)p.total_q * v_stride;  // one page of all rows
+    return attn_run_form(attn_tiles_fits(hd) ? ATTN_TILES : ATTN_WIDE, p, dtype, hd, p.total_q, 1, as_stream(stream));
 }
 
 }  // extern "C"

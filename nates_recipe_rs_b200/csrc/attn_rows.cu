@@ -558,33 +558,32 @@ static int attn_rows_inst(const AttnParams& p, const CUtensorMap& km, const CUte
     return QMM_OK;
 }
 
-template <int HD> static long ar_scratch_floats_hd(bool narrow) {
-    return narrow ? (long)ArScratch<HD, 16>::floats(sm_count() * ArShape<HD, 1>::CTAS_PER_SM) : (long)ArScratch<HD, 64>::floats(sm_count() * ArShape<HD, 4>::CTAS_PER_SM);
-}
+template <int HD, int WM> static long ar_scratch_bytes_of() { return 4 * (long)ArScratch<HD, 16 * WM>::floats(sm_count() * ArShape<HD, WM>::CTAS_PER_SM); }
 static long attn_rows_scratch_bytes(int hd, bool narrow) {
     switch (hd) {
-    case 32: return 4 * ar_scratch_floats_hd<32>(narrow);
-    case 64: return 4 * ar_scratch_floats_hd<64>(narrow);
-    case 96: return 4 * ar_scratch_floats_hd<96>(narrow);
-    case 128: return 4 * ar_scratch_floats_hd<128>(narrow);
-    case 256: return 4 * ar_scratch_floats_hd<256>(narrow);
+    case 32: return narrow ? ar_scratch_bytes_of<32, 1>() : ar_scratch_bytes_of<32, 4>();
+    case 64: return ar_scratch_bytes_of<64, 1>();
+    case 96: return ar_scratch_bytes_of<96, 1>();
+    case 128: return ar_scratch_bytes_of<128, 1>();
+    case 256: return narrow ? ar_scratch_bytes_of<256, 1>() : ar_scratch_bytes_of<256, 4>();
     }
     return QMM_ERR_UNSUPPORTED;
 }
-// CTAs that run at once: fewer items than this leave the GPU partly idle unless the items are shared
-static int attn_rows_slots(int hd) { return sm_count() * (hd <= 128 ? 2 : 1); }
 
-int attn_rows_launch(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, int dtype, int hd, bool narrow, cudaStream_t s) {
-#define QMM_AR_CASE(HD_)                                                                                                                       \
-    case HD_:                                                                                                                                  \
-        if (dtype == QMM_DT_F16) return narrow ? attn_rows_inst<__half, HD_, 1>(p, km, vm, s) : attn_rows_inst<__half, HD_, 4>(p, km, vm, s);  \
-        return narrow ? attn_rows_inst<__nv_bfloat16, HD_, 1>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, HD_, 4>(p, km, vm, s)
+// narrow: up to 16 rows per item; otherwise (head_dim 32 and 256 only: the others have attn_tiles.cu) 64
+static int attn_rows_launch(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, int dtype, int hd, bool narrow, cudaStream_t s) {
+    const bool f16 = dtype == QMM_DT_F16;
+#define QMM_AR_CASE(HD_, WM_) return f16 ? attn_rows_inst<__half, HD_, WM_>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, HD_, WM_>(p, km, vm, s)
     switch (hd) {
-        QMM_AR_CASE(32);
-        QMM_AR_CASE(64);
-        QMM_AR_CASE(96);
-        QMM_AR_CASE(128);
-        QMM_AR_CASE(256);
+    case 32:
+        if (narrow) QMM_AR_CASE(32, 1);
+        QMM_AR_CASE(32, 4);
+    case 64: QMM_AR_CASE(64, 1);
+    case 96: QMM_AR_CASE(96, 1);
+    case 128: QMM_AR_CASE(128, 1);
+    case 256:
+        if (narrow) QMM_AR_CASE(256, 1);
+        QMM_AR_CASE(256, 4);
     }
 #undef QMM_AR_CASE
     return QMM_ERR_UNSUPPORTED;
