@@ -71,10 +71,12 @@ static AttnForm attn_form(long max_q, int group, int hd) {
 }
 static int attn_run_form(AttnForm form, AttnParams& p, int dtype, int hd, long rows, long n_pages, cudaStream_t s) {
     const int tile = form == ATTN_TILES ? AT_TILE : AR_TILE;
-    p.box_rows = p.table ? gcd_int(p.page_size, tile) : tile;
+    const int box = p.table ? gcd_int(p.page_size, tile) : tile;  // pages are multiples of 8, tiles powers of two
+    for (p.box_shift = 3; 1 << p.box_shift < box;) ++p.box_shift;
+    p.group_inv = (65536 + p.group - 1) / p.group;
     CUtensorMap km, vm;
-    if (int st = kv_tensor_map(&km, p.k, dtype, hd, p.nkv, rows, n_pages, p.k_row, p.k_page, p.box_rows)) return st;
-    if (int st = kv_tensor_map(&vm, p.v, dtype, hd, p.nkv, rows, n_pages, p.v_row, p.v_page, p.box_rows)) return st;
+    if (int st = kv_tensor_map(&km, p.k, dtype, hd, p.nkv, rows, n_pages, p.k_row, p.k_page, box)) return st;
+    if (int st = kv_tensor_map(&vm, p.v, dtype, hd, p.nkv, rows, n_pages, p.v_row, p.v_page, box)) return st;
     if (form == ATTN_TILES) return attn_tiles_launch(p, km, vm, dtype, hd, s);
     return attn_rows_launch(p, km, vm, dtype, hd, form == ATTN_NARROW, s);
 }

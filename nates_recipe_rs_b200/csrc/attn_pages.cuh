@@ -28,7 +28,8 @@ struct AttnParams {
     int table_stride, page_size, n_pages;
     int n_seqs, total_q, max_kv;
     int nqh, nkv, group, window, out_dtype;
-    int box_rows;                            // rows of one tensor-map box: divides the tile and the page
+    int box_shift;                           // rows of one tensor-map box: 1 << box_shift, divides the tile and the page
+    int group_inv;                           // ceil(2^16 / group): r / group = r * group_inv >> 16 for the rows r < 256 of an item
     int stream_k;                            // 1: the CTAs share all (item, tile) pairs evenly and joined items go through scratch
     float scale_log2;                        // kq_scale * log2(e)
 };
@@ -39,8 +40,15 @@ struct SeqInfo {
 
 __device__ __forceinline__ void raise_status(int code) { atomicExch(&g_device_status, code); }
 
+// A bounded wait whose first probe alone is inlined: these kernels wait in many places, and their code has to fit the
+// instruction cache (items of a few tiles spent most of their time fetching code when everything was inlined and unrolled).
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* cta_abort) { return mbar_wait_bounded(bar, parity, cta_abort); }
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* cta_abort) {
+    return mbar_try_wait(smem_u32(bar), parity) || wait_slow(smem_u32(bar), parity, cta_abort);
+}
+
 // The lengths of a sequence, held inside the buffers whatever the arrays say (a value outside raises the device status).
-__device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int s) {
+__device__ __noinline__ SeqInfo seq_info(const AttnParams& p, int s) {
     const int a = p.cu_q[s], b = p.cu_q[s + 1];
     SeqInfo r;
     r.q0 = min(max(a, 0), p.total_q);
@@ -92,6 +100,7 @@ __device__ __forceinline__ int find_item(int n_seqs, long target, F f, long& bef
     long base = 0;
     int found = -1;
     long found_before = 0;
+#pragma unroll 1
     for (int s0 = 0; s0 < n_seqs; s0 += nt) {
         const int s = s0 + threadIdx.x;
         const long long v = s < n_seqs ? (long long)f(s) : 0ll;
@@ -105,6 +114,7 @@ __device__ __forceinline__ int find_item(int n_seqs, long target, F f, long& bef
         if (threadIdx.x == 0) sh[32] = -1;
         __syncthreads();
         long long wbase = base, all = 0;
+#pragma unroll 1
         for (int w = 0; w < nw; ++w) {
             if (w < warp) wbase += sh[w];
             all += sh[w];
@@ -145,15 +155,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 
-// A 32-bit word of two 16-bit values holds an infinity or a NaN
-template <typename T> __device__ __forceinline__ bool has_nonfinite(uint32_t w);
-template <> __device__ __forceinline__ bool has_nonfinite<__half>(uint32_t w) {
-    return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
-}
-template <> __device__ __forceinline__ bool has_nonfinite<__nv_bfloat16>(uint32_t w) {
-    return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
-}
-
 // Two neighbouring outputs (element index e, even) in the output's type
 __device__ __forceinline__ void store_out2(void* out, int dtype, size_t e, float a, float b) {
     if (dtype == QMM_DT_F32) *reinterpret_cast<float2*>(static_cast<float*>(out) + e) = make_float2(a, b);
@@ -174,40 +175,40 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(r), "r"(pg), "r"(bar)
                  : "memory");
 }
-// The boxes of tile `t` (TILE positions) that hold a key of [a, b): first, and how many
+// The boxes of tile `t` (TILE positions) that hold a key of [a, kv): first, and how many.  What no box covers, and what lies past
+// kv in the last one, is whatever was there before: the reader clears those rows (of the values; scores are masked).
 template <int TILE>
-__device__ __forceinline__ void tile_boxes(const AttnParams& p, int t, int a, int b, int& first, int& count) {
-    const int lo = max(a - t * TILE, 0), hi = min(b - t * TILE, TILE);
-    first = lo / p.box_rows;
-    count = hi > lo ? (hi - 1) / p.box_rows - first + 1 : 0;
+__device__ __forceinline__ void tile_boxes(const AttnParams& p, int t, int a, int kv, int& first, int& count) {
+    const int lo = max(a - t * TILE, 0), hi = min(kv - t * TILE, TILE);
+    first = lo >> p.box_shift;
+    count = hi > lo ? ((hi - 1) >> p.box_shift) - first + 1 : 0;
 }
 // Issued by a whole warp: the boxes of one matrix's tile.  `pages` holds, in lane j, the page of box j (page_of_boxes).
 template <int TILE, int NCH>
 __device__ __forceinline__ void load_tile(const AttnParams& p, const CUtensorMap* map, uint32_t dst, uint32_t bar, int t, int first, int count,
-                                          int pages, int row0, int kvh) {
+                                          int pages, int slots, int kvh) {
     const int lane = threadIdx.x & 31;
-    const int per_page = p.table ? p.page_size : 0;
-    for (int i = lane; i - lane < count * NCH; i += 32) {  // (the whole warp stays in the loop: the shuffle needs it)
+#pragma unroll 1
+    for (int i = lane; i - lane < count * NCH; i += 32) {  // (the whole warp stays in the loop: the shuffles need it)
         const int j = first + i / NCH, c = i % NCH;
-        const int pg = __shfl_sync(0xffffffffu, pages, j & 31);
-        if (i < count * NCH) {
-            const int pos = t * TILE + j * p.box_rows;
-            const int slot = per_page ? pos % per_page : row0 + pos;
-            tma_load_4d(dst + (uint32_t)(c * TILE + j * p.box_rows) * 128u, map, c * 64, kvh, slot, per_page ? pg : 0, bar);
-        }
+        const int pg = __shfl_sync(0xffffffffu, pages, j & 31), slot = __shfl_sync(0xffffffffu, slots, j & 31);
+        if (i < count * NCH) tma_load_4d(dst + (uint32_t)(c * TILE + (j << p.box_shift)) * 128u, map, c * 64, kvh, slot, pg, bar);
     }
 }
-// lane j: the page of box j of tile t (looked up ahead of the tile's turn)
+// lane j: page and slot of the first position of box j of tile t (looked up ahead of the tile's turn); packed rows are one page
 template <int TILE>
-__device__ __forceinline__ int page_of_boxes(const AttnParams& p, int s, int t, int first, int count) {
-    const int lane = threadIdx.x & 31;
+__device__ __forceinline__ int page_of_boxes(const AttnParams& p, int s, int row0, int t, int first, int count, int& slot) {
+    const int lane = threadIdx.x & 31, pos = t * TILE + (lane << p.box_shift);
+    slot = row0 + pos;
     if (!p.table || lane < first || lane >= first + count) return 0;
-    return page_of(p, s, (t * TILE + lane * p.box_rows) / p.page_size);
+    const int idx = pos / p.page_size;
+    slot = pos - idx * p.page_size;
+    return page_of(p, s, idx);
 }
 
 // ---- one row, exactly by the formula: keys [k0, k1) of those the row sees, one warp, lane l holds elements l + 32 j ----
-// The tensor cores add 0 * v for a masked key, which is not 0 when v is an infinity or a NaN; a tile that holds such a value
-// under a mask takes this path.  m is in units of the raw score.
+// The tensor cores add 0 * v for a masked key, which is not 0 when v is an infinity or a NaN: rows whose output is not finite are
+// computed again this way (where that is what the formula gives, it stays).  m is in units of the raw score.
 template <typename T, int HD>
 __device__ __noinline__ void attn_row_exact(const AttnParams& p, int s, int q0, int tok, int head, int kvh, int k0, int k1, float& m, float& l,
                                             float (&o)[HD / 32]) {
@@ -217,6 +218,7 @@ __device__ __noinline__ void attn_row_exact(const AttnParams& p, int s, int q0, 
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) qv[j] = to_f32<T>(qr[lane + 32 * j]), o[j] = 0.f;
     m = -INFINITY, l = 0.f;
+#pragma unroll 1
     for (int key = k0; key < k1; ++key) {
         size_t ko, vo;
         bool there = true;

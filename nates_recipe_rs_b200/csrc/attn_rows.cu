@@ -34,7 +34,8 @@ struct __align__(16) ArHeader {
     uint64_t full[8], empty[8];
     long long scan[36];
     float ml[4][16][2];
-    int abort_flag, nonfinite;
+    AttnParams p;  // a copy: functions that are not inlined would fetch the kernel's parameters from far away, one by one
+    int abort_flag;
 };
 
 template <int HD, int WM> constexpr size_t ar_smem_bytes() {
@@ -67,6 +68,12 @@ __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// a barrier of the math warps that tells all of them whether `x` holds for any thread
+__device__ __forceinline__ bool bar_any(bool x) {
+    int r;
+    asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %1, 0; barrier.cta.red.or.pred.aligned q, 1, 128, p; selp.b32 %0, 1, 0, q; }" : "=r"(r) : "r"((int)x) : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // Walks the segments (item, tiles [t0, t1) of it) of this CTA; every thread of the CTA runs it and gets the same segments.
@@ -94,7 +101,7 @@ struct ArWalker {
         const KeyRange kr = key_range(p, si, 0, si.q_len);
         return (long)((si.q_len * p.group + R - 1) / R) * p.nkv * max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - kr.a / AR_TILE);
     }
-    __device__ __forceinline__ bool next() {
+    __device__ __noinline__ bool next() {
         if (g >= g1) return false;
         while (item >= nrb * p.nkv) {  // (sequences without rows have no items)
             if (++s >= p.n_seqs) return false;
@@ -111,7 +118,7 @@ struct ArWalker {
     }
 };
 // First tile of CTA c of n when `total` tiles are shared evenly
-__device__ __forceinline__ long ar_share(long total, int c, int n) { return total * c / n; }
+__device__ __noinline__ long ar_share(long total, int c, int n) { return total * c / n; }
 constexpr int AR_MIN_TILES = 2;  // fewer tiles than this per CTA: fewer CTAs (a share of one tile costs more in joining than it saves)
 __device__ __forceinline__ int ar_ctas(long total, int grid) { return (int)max(1l, min((long)grid, total / AR_MIN_TILES)); }
 
@@ -124,7 +131,7 @@ template <int HD, int R> struct ArScratch {  // layout of the scratch: joins, th
 
 template <typename T, int HD, int WM>
 __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) attn_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                                                               const __grid_constant__ AttnParams p) {
+                                                               const __grid_constant__ AttnParams params) {
     using Sh = ArShape<HD, WM>;
     constexpr int R = 16 * WM, WN = 4 / WM, KW = AR_TILE / WN;  // rows of an item, warps along the keys, keys per warp and tile
     constexpr int NT = KW / 8, QPITCH = Sh::NCH * 64 + 8;
@@ -134,14 +141,17 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
     T* qs = reinterpret_cast<T*>(sm + (size_t)Sh::STAGES * 2 * Sh::TILE_BYTES);
     float* buf = reinterpret_cast<float*>(qs + R * QPITCH);  // (WM == 1) one 16 x HD output while the warps join
     ArHeader* hdr = reinterpret_cast<ArHeader*>(reinterpret_cast<uint8_t*>(buf) + (WM == 1 ? 16 * Sh::BUF_PITCH * 4 : 0));
+    const AttnParams& p = hdr->p;
     volatile int* cta_abort = &hdr->abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
         for (int i = 0; i < Sh::STAGES; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), 4);
-        hdr->abort_flag = 0, hdr->nonfinite = 0;
+        hdr->abort_flag = 0;
         mbar_fence_init();
     }
+    if (tid < (int)(sizeof(AttnParams) / 4)) reinterpret_cast<uint32_t*>(&hdr->p)[tid] = reinterpret_cast<const uint32_t*>(&params)[tid];
+    __syncthreads();
     pdl_wait_prior_grids();
     pdl_release_dependents();
 
@@ -194,28 +204,28 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
             int tok0, n_rows, t0, t1;
             KeyRange kr;
             block_range(tok0, n_rows, kr, t0, t1);
-            int first, count, pages = 0;
+            int first, count, slots = 0, pages = 0;
             if (t0 < t1) {
-                tile_boxes<AR_TILE>(p, t0, kr.a, kr.b, first, count);
-                pages = page_of_boxes<AR_TILE>(p, w.s, t0, first, count);
+                tile_boxes<AR_TILE>(p, t0, kr.a, w.si.kv, first, count);
+                pages = page_of_boxes<AR_TILE>(p, w.s, w.si.q0, t0, first, count, slots);
             }
             for (int t = t0; t < t1; ++t, ++it) {
                 const int st = it % Sh::STAGES;
-                int nfirst = 0, ncount = 0, npages = 0;
+                int nfirst = 0, ncount = 0, npages = 0, nslots = 0;
                 if (t + 1 < t1) {  // the next tile's pages are looked up before this tile's turn comes
-                    tile_boxes<AR_TILE>(p, t + 1, kr.a, kr.b, nfirst, ncount);
-                    npages = page_of_boxes<AR_TILE>(p, w.s, t + 1, nfirst, ncount);
+                    tile_boxes<AR_TILE>(p, t + 1, kr.a, w.si.kv, nfirst, ncount);
+                    npages = page_of_boxes<AR_TILE>(p, w.s, w.si.q0, t + 1, nfirst, ncount, nslots);
                 }
-                if (it >= Sh::STAGES && !mbar_wait_bounded(smem_u32(&hdr->empty[st]), ((it / Sh::STAGES) - 1) & 1, cta_abort)) {
+                if (it >= Sh::STAGES && !wait_bar(&hdr->empty[st], ((it / Sh::STAGES) - 1) & 1, cta_abort)) {
                     if (lane == 0) give_up(DEV_TIMEOUT_EMPTY);
                     break;
                 }
                 const uint32_t bar = smem_u32(&hdr->full[st]), dst = ring + (uint32_t)st * 2 * Sh::TILE_BYTES;
-                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)count * 2 * Sh::NCH * p.box_rows * 128);
+                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(count * 2 * Sh::NCH * 128) << p.box_shift);
                 __syncwarp();
-                load_tile<AR_TILE, Sh::NCH>(p, &kmap, dst, bar, t, first, count, pages, w.si.q0, w.kvh);
-                load_tile<AR_TILE, Sh::NCH>(p, &vmap, dst + Sh::TILE_BYTES, bar, t, first, count, pages, w.si.q0, w.kvh);
-                first = nfirst, count = ncount, pages = npages;
+                load_tile<AR_TILE, Sh::NCH>(p, &kmap, dst, bar, t, first, count, pages, slots, w.kvh);
+                load_tile<AR_TILE, Sh::NCH>(p, &vmap, dst + Sh::TILE_BYTES, bar, t, first, count, pages, slots, w.kvh);
+                first = nfirst, count = ncount, pages = npages, slots = nslots;
             }
         }
         // copies in flight land before the CTA ends (on every path: after a normal run the consumers have seen them all)
@@ -274,32 +284,19 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
 
         for (int t = t0; t < t1; ++t, ++it) {
             const int st = it % Sh::STAGES;
-            if (!mbar_wait_bounded(smem_u32(&hdr->full[st]), (it / Sh::STAGES) & 1, cta_abort)) {
+            if (!wait_bar(&hdr->full[st], (it / Sh::STAGES) & 1, cta_abort)) {
                 if (lane == 0) give_up(DEV_TIMEOUT_FULL);  // (on to the end all the same: the warps meet at barriers)
             }
             const uint32_t ks = ring + (uint32_t)st * 2 * Sh::TILE_BYTES, vs = ks + Sh::TILE_BYTES;
             const int k0 = t * AR_TILE;
             const bool masked = k0 < kr.a2 || k0 + AR_TILE > kr.b2;  // some row does not see some key of the tile
-            if (masked) {
-                // values that no row sees become zeros; where some row does not see a key, a value that is not finite
-                // does too, and the rows are computed again without the tensor cores (attn_row_exact)
-                uint8_t* vp = sm + (size_t)st * 2 * Sh::TILE_BYTES + Sh::TILE_BYTES;
-                bool odd = false;
+            const int c0 = ((kr.a >> p.box_shift) << p.box_shift) - k0, c1 = w.si.kv - k0;  // keys of the tile outside [c0, c1): not loaded
+            if (c0 > 0 || c1 < AR_TILE) {
+                uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)st * 2 * Sh::TILE_BYTES + Sh::TILE_BYTES);
                 for (int i = tid; i < Sh::NCH * AR_TILE * 8; i += 128) {
-                    const int key = k0 + ((i >> 3) % AR_TILE);
-                    if (key >= kr.a2 && key < kr.b2) continue;
-                    uint4* x = reinterpret_cast<uint4*>(vp) + i;
-                    if (key < kr.a || key >= kr.b) {
-                        *x = make_uint4(0u, 0u, 0u, 0u);
-                    } else {
-                        const uint4 y = *x;
-                        if (has_nonfinite<T>(y.x) || has_nonfinite<T>(y.y) || has_nonfinite<T>(y.z) || has_nonfinite<T>(y.w)) {
-                            *x = make_uint4(0u, 0u, 0u, 0u);
-                            odd = true;
-                        }
-                    }
+                    const int key = (i >> 3) % AR_TILE;
+                    if (key < c0 || key >= c1) vp[i] = make_uint4(0u, 0u, 0u, 0u);
                 }
-                if (odd) hdr->nonfinite = 1;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage is refilled by a copy
                 math_sync();
             }
@@ -396,17 +393,18 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
         auto row_sees = [&](int r) {  // row r has keys at all (else its output is 0)
             return w.si.kv - w.si.q_len + (r0 + r) / p.group >= 0;
         };
-        math_sync();  // every warp's verdict on the values
-        const bool exact = hdr->nonfinite != 0;
-        math_sync();
-        if (exact) {
-            if (tid == 0) hdr->nonfinite = 0;
+        // outputs that are not finite: from a value that the row does not see, or by the formula; either way again, exactly
+        float odd = 0.f;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) odd += (o[n][0] + o[n][1]) * 0.f + (o[n][2] + o[n][3]) * 0.f;
+        if (bar_any(odd != odd)) {
+#pragma unroll 1
             for (int r = warp; r < n_rows; r += 4) {
                 const int tok = (r0 + r) / p.group, pos = w.si.kv - w.si.q_len + tok;
                 float em, el, eo[HD / 32];
                 attn_row_exact<T, HD>(p, w.s, w.si.q0, tok, w.kvh * p.group + (r0 + r) % p.group, w.kvh,
                                       max(w.t0 * AR_TILE, p.window ? max(0, pos - p.window + 1) : 0), min(w.t1 * AR_TILE, pos + 1), em, el, eo);
-                const float inv = row_sees(r) ? 1.f / el : 0.f;
+                const float inv = 1.f / el;
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) {
                     if (whole) store_out1(p.out, p.out_dtype, out_elem(r) + lane + 32 * j, row_sees(r) ? eo[j] * inv : 0.f);

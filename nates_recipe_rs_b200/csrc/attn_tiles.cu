@@ -5,22 +5,28 @@
 // one tile of keys and values serves every query head that shares it and a tile spans few positions (128 / group tokens: little
 // of the causal triangle is computed and thrown away).  For every tile of 128 keys and each of the two row tiles
 //     S = Q K^T    128 x 128 x HD, both operands in shared memory, S in tensor memory (f32)
-//     P = exp2((S - m) * c), row sums            one thread per row, S read with tcgen05.ld, P written back over S (16 bit)
+//     P = exp2((S - m) * c), row sums            in registers, S read with tcgen05.ld, P written back over S (16 bit)
 //     O += P V     128 x HD x 128, P from tensor memory, V from shared memory as it arrives (keys are the K dimension: the
 //                  operand is "MN major"), O in tensor memory for the whole run over the keys
 // While the threads of one row tile compute exponentials the tensor cores work for the other: the two pipes (16 exponentials per
 // clock and SM; 8192 flops) need about the same time at HD = 128.  The running maximum that P is scaled by is only moved when a
 // row's maximum has grown by more than 2^8 (P <= 256 fits f16, l and O are f32): O is rescaled in tensor memory a few times per
 // run instead of once per tile, with no separate correction step.
-// Warps: 0-3 and 4-7 softmax of row tile 0 / 1 (and its epilogue); 8 issues the tcgen05.mma; 9 issues the TMA copies (queries,
-// and keys and values through a ring of 128-key slots); 10-11 clear what no row sees out of the value tiles that need it.
+// Warps: 0-7 and 8-15 softmax of row tile 0 / 1 (and its epilogue), 16 rows each, a row in four lanes: with a thread per row, four
+// warps per tile, a warp had no one to share its scheduler with and issued every third cycle; 16 and 19 issue the tcgen05.mma of
+// row tile 0 / 1 (an issuing thread blocks while the tensor cores are busy, and every wait or commit costs it some 90 cycles more:
+// with one issuer for both tiles these were idle time of the tensor cores); 17 issues the TMA copies (queries, and keys and values
+// through a ring of 128-key slots); 18 clears what no row sees out of the value tiles that need it.
+// The CTAs stay: each takes items until none is left, so that the copies and the scores of the next item run under the epilogue
+// of the one before (a CTA per item spent 7 us between the last tile of one and the first of the next).
 // Every wait is bounded; on expiry the CTA records a status code, drains its copies, frees its tensor memory and returns.
 #include "attn_pages.cuh"
 
 namespace qmm {
 
 constexpr int AT_TILE = 128;  // keys per tile, and rows per tile
-constexpr int AT_THREADS = 384;
+constexpr int AT_THREADS = 640;  // 16 softmax warps, two issuing warps, the copying and the clearing warp
+constexpr int AT_WARP_MMA0 = 16, AT_WARP_COPY = 17, AT_WARP_CLEAR = 18, AT_WARP_MMA1 = 19;
 constexpr int AT_MAX_ROWS = 256;  // rows of an item
 template <int HD> struct AtShape {
     static constexpr int NCH = (HD + 63) / 64;
@@ -29,14 +35,17 @@ template <int HD> struct AtShape {
     __host__ __device__ static constexpr uint32_t IDESC_S(bool bf16) { return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((AT_TILE >> 3) << 17) | ((128 >> 4) << 24); }
     __host__ __device__ static constexpr uint32_t IDESC_O(bool bf16) { return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24); }
 };
-constexpr uint32_t AT_COL_S = 0, AT_COL_O = 256;  // tensor memory columns: S (and P over it) of tile i at 128 i, O at 256 + 128 i
+// tensor memory columns: S of tile i at 128 i, P over the second half of S (the half that is read last goes there first), O of
+// tile i at 256 + 128 i
+constexpr uint32_t AT_COL_S = 0, AT_COL_P = 64, AT_COL_O = 256;
 
 struct __align__(16) AtHeader {
     uint64_t full[10], empty[10];
-    uint64_t v_ask, v_ok, q_full, q_empty, s_full[2], p_full[2], o_full[2], drain;
+    uint64_t v_ask, v_ok, q_full, q_empty, s_full[2], p_part[2], p_full[2], o_full[2], turn[2][4], drain[2];
     long long scan[36];
+    AttnParams p;  // a copy: functions that are not inlined would fetch the kernel's parameters from far away, one by one
     uint32_t tmem_base;
-    int abort_flag, nonfinite;
+    int abort_flag;
 };
 template <int HD> constexpr size_t at_smem_bytes() { return 1024 + (size_t)(2 + AtShape<HD>::SLOTS) * AtShape<HD>::TILE_BYTES + sizeof(AtHeader); }
 
@@ -53,55 +62,137 @@ __device__ __forceinline__ uint64_t umma_desc_v(uint32_t smem_addr) {
 }
 #define QMM_R8(r, b) "=r"(r[b]), "=r"(r[b + 1]), "=r"(r[b + 2]), "=r"(r[b + 3]), "=r"(r[b + 4]), "=r"(r[b + 5]), "=r"(r[b + 6]), "=r"(r[b + 7])
 #define QMM_RI8(r, b) "r"(r[b]), "r"(r[b + 1]), "r"(r[b + 2]), "r"(r[b + 3]), "r"(r[b + 4]), "r"(r[b + 5]), "r"(r[b + 6]), "r"(r[b + 7])
-// 128 columns of this warp's 32 lanes.  The wait is part of the statement: between a load and its wait nothing may touch the
-// registers, not even a spill that the compiler puts there.
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+// Tensor memory by 16 rows (lanes 0-15 or 16-31 of the warp's quarter): lane l of the warp holds, of each block of 8 columns, columns
+// 2 (l & 3) and + 1 of rows l / 4 (registers 4 i, 4 i + 1 of block i) and l / 4 + 8 (4 i + 2, 4 i + 3): a row lies in four lanes.
+// The wait is part of a load: between a load and its wait nothing may touch the registers, not even a spill that the compiler
+// puts there.
+__device__ __forceinline__ void tmem_ld_8(uint32_t taddr, uint32_t (&r)[32]) {  // 64 columns
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
-        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-        "%28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, "
-        "%54, %55, %56, %57, %58, %59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
-        "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, "
-        "%105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126"
-        ", %127"
-        "}, [%128];\n\t"
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : QMM_R8(r, 0), QMM_R8(r, 8), QMM_R8(r, 16), QMM_R8(r, 24), QMM_R8(r, 32), QMM_R8(r, 40), QMM_R8(r, 48), QMM_R8(r, 56), QMM_R8(r, 64), QMM_R8(r, 72), QMM_R8(r, 80), QMM_R8(r, 88), QMM_R8(r, 96), QMM_R8(r, 104), QMM_R8(r, 112), QMM_R8(r, 120)
+        : QMM_R8(r, 0), QMM_R8(r, 8), QMM_R8(r, 16), QMM_R8(r, 24)
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::QMM_RI8(r, 0),
+__device__ __forceinline__ void tmem_ld_4(uint32_t taddr, uint32_t (&r)[16]) {  // 32 columns
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : QMM_R8(r, 0), QMM_R8(r, 8)
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_4(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::QMM_RI8(r, 0),
                  QMM_RI8(r, 8), "r"(taddr)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::QMM_RI8(r, 0),
-        QMM_RI8(r, 8), QMM_RI8(r, 16), QMM_RI8(r, 24), "r"(taddr)
-        : "memory");
+// 16-bit pairs: 4 columns of 32 bits per block of 8 values; registers 2 i (row l / 4) and 2 i + 1 (row l / 4 + 8), column l & 3
+__device__ __forceinline__ void tmem_st_p(uint32_t taddr, const uint32_t (&r)[16]) {  // 64 values a row: 32 columns
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::QMM_RI8(r, 0),
+                 QMM_RI8(r, 8), "r"(taddr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // one instruction; a NaN is ignored, as by fmaxf
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
 
-// The segments (item, tiles [t0, t1) of it) of this CTA.  An item is (sequence, kv head, block of tb tokens); where the tiles are
-// shared evenly, every item of a sequence counts as many as the sequence's last block has, at least one.
+// Scores of 64 keys from k0 on (this lane's columns of two rows): those from hi[e] on / before lo[e] do not count for row e
+__device__ __forceinline__ void mask_right(uint32_t (&s)[32], int k0, const int (&hi)[2]) {
+    const int n[2] = {hi[0] - k0 - 2 * ((int)threadIdx.x & 3), hi[1] - k0 - 2 * ((int)threadIdx.x & 3)};
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+        if (8 * (j >> 2) + (j & 1) >= n[(j >> 1) & 1]) s[j] = 0xFF800000u;  // -inf
+}
+__device__ __forceinline__ void mask_left(uint32_t (&s)[32], int k0, const int (&lo)[2]) {
+    const int n[2] = {lo[0] - k0 - 2 * ((int)threadIdx.x & 3), lo[1] - k0 - 2 * ((int)threadIdx.x & 3)};
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+        if (8 * (j >> 2) + (j & 1) < n[(j >> 1) & 1]) s[j] = 0xFF800000u;
+}
+__device__ __forceinline__ void max64(const uint32_t (&s)[32], float (&m)[2]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) m[e] = max3(m[e], __uint_as_float(s[j + 2 * e]), __uint_as_float(s[j + 2 * e + 1]));
+}
+// Two f32 operations at a time
+__device__ __forceinline__ uint64_t f32x2(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float lo2(uint64_t a) { return __uint_as_float((uint32_t)a); }
+__device__ __forceinline__ float hi2(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
+// P = exp2(s c - mc) of 64 keys to 32 columns of tensor memory; adds this lane's columns to l (before they are rounded)
+template <typename T>
+__device__ __forceinline__ void exp64(const uint32_t (&s)[32], float c, const float (&mc)[2], uint32_t tp, uint64_t (&l)[2]) {
+    const uint64_t c2 = f32x2(c, c);
+    uint32_t pk[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int e = j & 1;
+        const uint64_t x = fma2(f32x2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), c2, f32x2(-mc[e], -mc[e]));
+        const uint64_t y = f32x2(fast_exp2(lo2(x)), fast_exp2(hi2(x)));
+        l[e] = add2(l[e], y);
+        pk[j] = pack2<T>(lo2(y), hi2(y));
+    }
+    tmem_st_p(tp, pk);
+}
+
+// Four words per lane in four lanes: afterwards lane j of the four holds word j of every lane, in lane order
+__device__ __forceinline__ void turn4(uint32_t (&v)[4]) {
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) {
+        const bool up = threadIdx.x & d;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k & d) continue;
+            const uint32_t x = __shfl_xor_sync(0xffffffffu, up ? v[k] : v[k + d], d);
+            if (up) v[k] = x;
+            else v[k + d] = x;
+        }
+    }
+}
+
+// The segments (item, tiles [t0, t1) of it) of this CTA; every warp of the CTA walks them (whole warps, all lanes alike).  An item
+// is (sequence, kv head, block of tb tokens).
+// Many items: whole items, CTA c of n takes number c, 2n-1-c, 2n+c, ... of all (a sequence's last, longest blocks first, every
+// second round backwards: the rounds' differences cancel).  Few items over a long axis (stream_k): all tiles are shared evenly in
+// order, where every item of a sequence counts as many tiles as its last block has, at least one.
 struct AtWalker {
     const AttnParams& p;
     int tb;        // tokens per block
-    long g, g1;
+    int left;      // stream_k: tiles of this CTA's share still to come; else 0 after the last item
+    int ahead, turn;  // items from the current one to the next, rounds so far
     int s, item, within;
     SeqInfo si;
     int tl, nt, nb;
     // the current segment
     int kvh, tok0, tok1, t0, t1;  // tokens [tok0, tok1), tiles [t0, t1) that hold keys of its rows
     int st0, st1;                 // tiles of the segment before that cut
+    int u0, u1;                   // tiles [u0, u1) whose keys every row sees
+    int d0, d1;                   // tiles [d0, d1) that are loaded whole
     bool begins, ends;
     KeyRange kr;
 
@@ -115,57 +206,132 @@ struct AtWalker {
         nt = count(si, r);
         nb = (si.q_len + tb - 1) / tb;
     }
+    __device__ static __forceinline__ int items_of(const AttnParams& p, int tb, int s) { return (seq_info(p, s).q_len + tb - 1) / tb * p.nkv; }
     __device__ static __forceinline__ long tiles_of(const AttnParams& p, int tb, int s) {
         const SeqInfo si = seq_info(p, s);
         return (long)((si.q_len + tb - 1) / tb) * p.nkv * count(si, key_range(p, si, 0, si.q_len));
     }
-    __device__ __forceinline__ bool next() {
-        if (g >= g1) return false;
-        while (item >= nb * p.nkv) {
-            if (++s >= p.n_seqs) return false;
-            item = within = 0;
-            load_seq();
+    // To the item `n` after the current one; 32 sequences are looked at at a time.
+    __device__ __forceinline__ bool skip(int n) {
+        const int lane = threadIdx.x & 31;
+        int target = item + n;
+        if (target >= nb * p.nkv) {
+            target -= nb * p.nkv;
+            for (int base = s + 1;; base += 32) {
+                if (base >= p.n_seqs) return false;
+                const int cnt = base + lane < p.n_seqs ? items_of(p, tb, base + lane) : 0;
+                int inc = cnt;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += u;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, inc > target);
+                if (past) {
+                    const int f = __ffs(past) - 1;
+                    s = base + f;
+                    target -= __shfl_sync(0xffffffffu, inc - cnt, f);
+                    load_seq();
+                    break;
+                }
+                target -= __shfl_sync(0xffffffffu, inc, 31);
+            }
         }
-        const int n = (int)min(g1 - g, (long)(nt - within));
-        kvh = item / nb;
-        tok0 = (item - kvh * nb) * tb, tok1 = min(tok0 + tb, si.q_len);
-        st0 = tl + within, st1 = st0 + n;
-        begins = within == 0, ends = within + n == nt;
-        kr = key_range(p, si, tok0, tok1);
-        t0 = max(st0, kr.a / AT_TILE), t1 = min(st1, (kr.b + AT_TILE - 1) / AT_TILE);
-        g += n, within += n;
-        if (within == nt) within = 0, ++item;
+        item = target;
         return true;
     }
-    // some row of the segment does not see some key of tile t
-    __device__ __forceinline__ bool masked(int t) const { return t * AT_TILE < kr.a2 || (t + 1) * AT_TILE > kr.b2; }
+    // (not inlined: five roles call it, and code that runs once per item should not push the loops out of the instruction cache)
+    __device__ __noinline__ bool next() {
+        if (left <= 0) return false;
+        int blk;
+        if (p.stream_k) {
+            while (item >= nb * p.nkv) {
+                if (++s >= p.n_seqs) return false;
+                item = within = 0;
+                load_seq();
+            }
+            const int n = min(left, nt - within);
+            kvh = item / nb, blk = item - kvh * nb;
+            st0 = tl + within, st1 = st0 + n;
+            begins = within == 0, ends = within + n == nt;
+            left -= n, within += n;
+            if (within == nt) within = 0, ++item;
+        } else {
+            if (!skip(ahead)) {
+                left = 0;
+                return false;
+            }
+            const int n = gridDim.x, c = blockIdx.x;
+            ahead = (turn++ & 1) ? 2 * c + 1 : 2 * (n - c) - 1;
+            blk = item / p.nkv, kvh = item - blk * p.nkv, blk = nb - 1 - blk;
+            st0 = tl, st1 = tl + nt;
+            begins = ends = true;
+        }
+        tok0 = blk * tb, tok1 = min(tok0 + tb, si.q_len);
+        kr = key_range(p, si, tok0, tok1);
+        t0 = max(st0, kr.a / AT_TILE), t1 = min(st1, (kr.b + AT_TILE - 1) / AT_TILE);
+        u0 = (kr.a2 + AT_TILE - 1) / AT_TILE, u1 = kr.b2 / AT_TILE;
+        d0 = (((kr.a >> p.box_shift) << p.box_shift) + AT_TILE - 1) / AT_TILE, d1 = si.kv / AT_TILE;
+        return true;
+    }
+    // rows of value tile t were not loaded, or are not of this sequence
+    __device__ __forceinline__ bool dirty(int t) const { return t < d0 || t >= d1; }
 };
+
+// The 16 rows of a warp (rows row0 .. row0 + 15 of the row tile whose first token is tok0 of the block) without the tensor cores
+template <typename T, int HD>
+__device__ __noinline__ void at_exact_rows(const AttnParams& p, const AtWalker& w, int tok0, int row0, int tile_rows, bool whole, float* so, float* ml) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int row = row0; row < row0 + 16; ++row) {
+        const int tok = w.tok0 + tok0 + row / p.group, pos = w.si.kv - w.si.q_len + tok, head = w.kvh * p.group + row % p.group;
+        if (row >= tile_rows || tok >= w.tok1) break;
+        float m, l, o[HD / 32];
+        attn_row_exact<T, HD>(p, w.s, w.si.q0, tok, head, w.kvh, max(w.st0 * AT_TILE, p.window ? max(0, pos - p.window + 1) : 0),
+                              min(w.st1 * AT_TILE, pos + 1), m, l, o);
+        const int r = (tok - w.tok0) * p.group + row % p.group;
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+            if (whole) store_out1(p.out, p.out_dtype, (size_t)(w.si.q0 + tok) * p.out_stride + (size_t)head * HD + lane + 32 * j, pos >= 0 ? o[j] * inv : 0.f);
+            else so[(size_t)r * HD + lane + 32 * j] = o[j];
+        }
+        if (!whole && lane == 0) ml[2 * r] = m, ml[2 * r + 1] = l;
+    }
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                                                                   const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p) {
+                                                                   const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams params) {
     using Sh = AtShape<HD>;
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(1024) uint8_t at_raw[];
     uint8_t* sm = at_raw + ((1024u - (smem_u32(at_raw) & 1023u)) & 1023u);
     const uint32_t q_s = smem_u32(sm), ring = q_s + 2 * Sh::TILE_BYTES;
     AtHeader* hdr = reinterpret_cast<AtHeader*>(sm + (size_t)(2 + Sh::SLOTS) * Sh::TILE_BYTES);
+    const AttnParams& p = hdr->p;
     volatile int* cta_abort = &hdr->abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int tpt = AT_TILE / p.group, tile_rows = tpt * p.group;  // tokens and rows of a row tile
+    const int tpt = AT_TILE / params.group, tile_rows = tpt * params.group;  // tokens and rows of a row tile
 
     if (tid == 0) {
-        for (int i = 0; i < Sh::SLOTS; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), 1);
-        mbar_init(smem_u32(&hdr->v_ask), 1), mbar_init(smem_u32(&hdr->v_ok), 2);
-        mbar_init(smem_u32(&hdr->q_full), 1), mbar_init(smem_u32(&hdr->q_empty), 1), mbar_init(smem_u32(&hdr->drain), 1);
-        for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&hdr->s_full[i]), 1), mbar_init(smem_u32(&hdr->p_full[i]), 4), mbar_init(smem_u32(&hdr->o_full[i]), 1);
-        hdr->abort_flag = 0, hdr->nonfinite = 0;
+        for (int i = 0; i < Sh::SLOTS; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), 2);
+        mbar_init(smem_u32(&hdr->v_ask), 2), mbar_init(smem_u32(&hdr->v_ok), 1);
+        mbar_init(smem_u32(&hdr->q_full), 1), mbar_init(smem_u32(&hdr->q_empty), 2);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&hdr->s_full[i]), 1), mbar_init(smem_u32(&hdr->o_full[i]), 1), mbar_init(smem_u32(&hdr->drain[i]), 1);
+            mbar_init(smem_u32(&hdr->p_part[i]), 8), mbar_init(smem_u32(&hdr->p_full[i]), 8);
+            for (int j = 0; j < 4; ++j) mbar_init(smem_u32(&hdr->turn[i][j]), 2);
+        }
+        hdr->abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == 8) {
+    if (warp == AT_WARP_MMA0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hdr->tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (tid < (int)(sizeof(AttnParams) / 4)) reinterpret_cast<uint32_t*>(&hdr->p)[tid] = reinterpret_cast<const uint32_t*>(&params)[tid];
+    __syncthreads();
     pdl_wait_prior_grids();
     pdl_release_dependents();
 
@@ -177,24 +343,29 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         find_item(p.n_seqs, 1l << 62, [&](int s) { return AtWalker::tiles_of(p, 2 * tpt, s); }, total, hdr->scan);
         n_ctas = ar_ctas(total, gridDim.x);
         if (tid == 0) (reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x)->n_rows = 0;
-        w.g = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas), w.g1 = ar_share(total, min((int)blockIdx.x + 1, n_ctas), n_ctas);
-        w.s = find_item(p.n_seqs, w.g, [&](int s) { return AtWalker::tiles_of(p, 2 * tpt, s); }, before, hdr->scan);
+        const long g = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
+        w.left = (int)(ar_share(total, min((int)blockIdx.x + 1, n_ctas), n_ctas) - g);
+        w.s = find_item(p.n_seqs, g, [&](int s) { return AtWalker::tiles_of(p, 2 * tpt, s); }, before, hdr->scan);
         any = (int)blockIdx.x < n_ctas && w.s >= 0;
         if (any) {
             w.load_seq();
-            w.item = (int)((w.g - before) / w.nt), w.within = (int)((w.g - before) % w.nt);
+            w.item = (int)((g - before) / w.nt), w.within = (int)((g - before) % w.nt);
         }
     } else {
-        // one item per CTA: block blockIdx.y of all blocks (a sequence's last, longest, first), kv head blockIdx.x
-        w.s = find_item(p.n_seqs, blockIdx.y, [&](int s) { return (long)((seq_info(p, s).q_len + 2 * tpt - 1) / (2 * tpt)); }, before, hdr->scan);
-        any = w.s >= 0;
-        if (any) {
-            w.load_seq();
-            w.g = 0, w.g1 = w.nt, w.within = 0;
-            w.item = blockIdx.x * w.nb + (w.nb - 1 - (int)(blockIdx.y - before));
+        // whole items: the first is number blockIdx.x (few sequences: the walk finds it by itself)
+        any = true;
+        w.s = -1, w.item = w.nb = w.within = 0, w.left = 1, w.ahead = blockIdx.x, w.turn = 0;
+        if (p.n_seqs > 64) {
+            w.s = find_item(p.n_seqs, blockIdx.x, [&](int s) { return AtWalker::items_of(p, 2 * tpt, s); }, before, hdr->scan);
+            any = w.s >= 0;
+            if (any) {
+                w.load_seq();
+                w.item = (int)(blockIdx.x - before), w.ahead = 0;
+            }
         }
     }
-    if (!any) w.g = w.g1 = 0;
+    if (!any) w.left = 0;
+    if (tid == 0) hdr->scan[34] = total, hdr->scan[35] = n_ctas;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -207,19 +378,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         }
     };
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
-        if (mbar_wait_bounded(smem_u32(bar), phase & 1u, cta_abort)) return true;
+        if (wait_bar(bar, phase & 1u, cta_abort)) return true;
         give_up(code);
         return false;
     };
 
 
-    if (warp == 9) {
+    if (warp == AT_WARP_COPY) {
         // ------------------------------------------------------------ copies
         int it = 0, q_no = 0;  // tiles (of keys and of values) and query blocks so far
         bool ok = true;
         while (ok && w.next()) {
             if (w.t0 >= w.t1) continue;
             const int nq = w.tok1 - w.tok0 > tpt ? 2 : 1;
+            int first, cnt, pages, slots;
+            tile_boxes<AT_TILE>(p, w.t0, w.kr.a, w.si.kv, first, cnt);
+            pages = page_of_boxes<AT_TILE>(p, w.s, w.si.q0, w.t0, first, cnt, slots);
             if (q_no > 0 && !wait(&hdr->q_empty, q_no - 1, DEV_TIMEOUT_EMPTY)) break;
             if (lane == 0) mbar_arrive_expect_tx(smem_u32(&hdr->q_full), (uint32_t)(nq * Sh::NCH * tile_rows * 128));
             __syncwarp();
@@ -229,16 +403,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                             smem_u32(&hdr->q_full));
             }
             ++q_no;
-            int first, cnt, pages;
-            tile_boxes<AT_TILE>(p, w.t0, w.kr.a, w.kr.b, first, cnt);
-            pages = page_of_boxes<AT_TILE>(p, w.s, w.t0, first, cnt);
             for (int t = w.t0; t < w.t1 && ok; ++t) {
-                int nfirst = 0, ncnt = 0, npages = 0;
+                int nfirst = 0, ncnt = 0, npages = 0, nslots = 0;
                 if (t + 1 < w.t1) {  // the next tile's pages are looked up before its turn comes
-                    tile_boxes<AT_TILE>(p, t + 1, w.kr.a, w.kr.b, nfirst, ncnt);
-                    npages = page_of_boxes<AT_TILE>(p, w.s, t + 1, nfirst, ncnt);
+                    tile_boxes<AT_TILE>(p, t + 1, w.kr.a, w.si.kv, nfirst, ncnt);
+                    npages = page_of_boxes<AT_TILE>(p, w.s, w.si.q0, t + 1, nfirst, ncnt, nslots);
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv, ++it) {
                     const int sl = it % Sh::SLOTS;
                     if (it >= Sh::SLOTS && !wait(&hdr->empty[sl], it / Sh::SLOTS - 1, DEV_TIMEOUT_EMPTY)) {
@@ -246,14 +417,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                         break;
                     }
                     const uint32_t bar = smem_u32(&hdr->full[sl]);
-                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)cnt * Sh::NCH * p.box_rows * 128);
+                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(cnt * Sh::NCH * 128) << p.box_shift);
                     __syncwarp();
-                    load_tile<AT_TILE, Sh::NCH>(p, kv ? &vmap : &kmap, ring + (uint32_t)sl * Sh::TILE_BYTES, bar, t, first, cnt, pages, w.si.q0, w.kvh);
+                    load_tile<AT_TILE, Sh::NCH>(p, kv ? &vmap : &kmap, ring + (uint32_t)sl * Sh::TILE_BYTES, bar, t, first, cnt, pages, slots, w.kvh);
                 }
-                first = nfirst, cnt = ncnt, pages = npages;
+                first = nfirst, cnt = ncnt, pages = npages, slots = nslots;
             }
         }
         if (*cta_abort) {  // copies in flight land before the CTA ends
+#pragma unroll 1
             for (int i = max(0, it - Sh::SLOTS); i <= it; ++i) {
                 uint64_t* bar = i < it ? &hdr->full[i % Sh::SLOTS] : &hdr->q_full;
                 const uint32_t ph = i < it ? (i / Sh::SLOTS) & 1 : (q_no - 1) & 1;
@@ -266,139 +438,149 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                     }
             }
         }
-    } else if (warp == 8) {
-        // ------------------------------------------------------------ tensor cores (one thread)
-        if (lane == 0) {
-            int it = 0, q_no = 0;
-            uint32_t n_p[2] = {0, 0};  // P tiles awaited so far, per row tile
-            uint32_t n_v = 0;          // value tiles handed to the clearing warps so far
-            bool ok = true;
-            auto mma_s = [&](int i, int slot) {
-                const uint64_t qd = umma_desc_sw128(q_s + (uint32_t)i * Sh::TILE_BYTES), kd = umma_desc_sw128(ring + (uint32_t)slot * Sh::TILE_BYTES);
+    } else if (warp == AT_WARP_MMA0 || warp == AT_WARP_MMA1) {
+        // ------------------------------------------------------------ tensor cores: row tile i (one thread issues)
+        // Both issuers follow every segment and every slot, also where there is no second row tile: a barrier whose phases one of
+        // them skipped could not be waited for by parity.
+        const int i = warp == AT_WARP_MMA0 ? 0 : 1;
+        const uint32_t d_s = tmem + AT_COL_S + 128u * i, d_o = tmem + AT_COL_O + 128u * i;
+        const uint64_t qd = umma_desc_sw128(q_s + (uint32_t)i * Sh::TILE_BYTES);
+        int it = 0, q_no = 0;
+        uint32_t n_p = 0, n_v = 0;  // P tiles awaited, value tiles handed to the clearing warp so far
+        bool ok = true, active = false;
+        auto mma_s = [&](int slot) {
+            const uint64_t kd = umma_desc_sw128(ring + (uint32_t)slot * Sh::TILE_BYTES);
 #pragma unroll
-                for (int k16 = 0; k16 < HD / 16; ++k16) {  // 32 bytes of a 128-byte row each; the next 64 elements one chunk further
-                    const uint64_t off = (uint64_t)((k16 >> 2) * (AT_TILE * 128 >> 4) + (k16 & 3) * 2);
-                    umma_bf16(tmem + AT_COL_S + 128u * i, qd + off, kd + off, Sh::IDESC_S(BF16), k16 > 0);
-                }
-                umma_commit(smem_u32(&hdr->s_full[i]));
-            };
-            auto mma_o = [&](int i, int slot, bool acc) {
-                const uint64_t vd = umma_desc_v(ring + (uint32_t)slot * Sh::TILE_BYTES);
+            for (int k16 = 0; k16 < HD / 16; ++k16) {  // 32 bytes of a 128-byte row each; the next 64 elements one chunk further
+                const uint64_t off = (uint64_t)((k16 >> 2) * (AT_TILE * 128 >> 4) + (k16 & 3) * 2);
+                umma_bf16(d_s, qd + off, kd + off, Sh::IDESC_S(BF16), k16 > 0);
+            }
+            umma_commit(smem_u32(&hdr->s_full[i]));
+        };
+        auto mma_o = [&](int slot, int first, int last, bool acc) {  // 16 keys each: 8 columns of P, 2048 bytes of V
+            const uint64_t vd = umma_desc_v(ring + (uint32_t)slot * Sh::TILE_BYTES);
 #pragma unroll
-                for (int k16 = 0; k16 < AT_TILE / 16; ++k16)  // 16 keys: 8 columns of P, 2048 bytes of V
-                    umma_ts(tmem + AT_COL_O + 128u * i, tmem + AT_COL_S + 128u * i + 8u * k16, vd + (uint64_t)(k16 * (2048 >> 4)), Sh::IDESC_O(BF16),
-                            (acc || k16 > 0) ? 1u : 0u);
-            };
-            // a value tile with keys that some row does not see goes through the clearing warps while its scores are in softmax
-            auto ask_v = [&](int t, int v_it) {
-                if (!w.masked(t)) return true;
-                if (!wait(&hdr->full[v_it % Sh::SLOTS], v_it / Sh::SLOTS, DEV_TIMEOUT_FULL)) return false;
-                mbar_arrive(smem_u32(&hdr->v_ask));
-                ++n_v;
-                return true;
-            };
-            while (ok && w.next()) {
-                if (w.t0 >= w.t1) continue;
-                const int nq = w.tok1 - w.tok0 > tpt ? 2 : 1;
-                if (!wait(&hdr->q_full, q_no, DEV_TIMEOUT_FULL)) break;
-                ++q_no;
-                int sl = it % Sh::SLOTS;
-                if (!wait(&hdr->full[sl], it / Sh::SLOTS, DEV_TIMEOUT_FULL)) break;
-                tc_fence_after();
-                for (int i = 0; i < nq; ++i) mma_s(i, sl);
-                umma_commit(smem_u32(&hdr->empty[sl]));
-                if (w.t0 + 1 == w.t1) umma_commit(smem_u32(&hdr->q_empty));
-                ++it;
-                ok = ask_v(w.t0, it);
-                for (int t = w.t0; t < w.t1 && ok; ++t) {
-                    const int vs = it % Sh::SLOTS, ks = (it + 1) % Sh::SLOTS;
-                    const bool more = t + 1 < w.t1;
-                    ok = wait(&hdr->full[vs], it / Sh::SLOTS, DEV_TIMEOUT_FULL);
-                    if (ok && w.masked(t)) ok = wait(&hdr->v_ok, n_v - 1, DEV_TIMEOUT_FULL);
-                    if (ok && more) ok = wait(&hdr->full[ks], (it + 1) / Sh::SLOTS, DEV_TIMEOUT_FULL);
-                    for (int i = 0; i < nq && ok; ++i) {
-                        ok = wait(&hdr->p_full[i], n_p[i], DEV_TIMEOUT_MMA);
-                        if (!ok) break;
-                        ++n_p[i];
-                        tc_fence_after();
-                        mma_o(i, vs, t > w.t0);
-                        if (more) mma_s(i, ks);
+            for (int k16 = first; k16 < last; ++k16)
+                umma_ts(d_o, d_s + AT_COL_P + 8u * k16, vd + (uint64_t)(k16 * (2048 >> 4)), Sh::IDESC_O(BF16), (acc || k16 > first) ? 1u : 0u);
+        };
+        auto release = [&](uint64_t* bar) {  // when what this thread has issued so far retires
+            if (lane == 0) {
+                if (active) umma_commit(smem_u32(bar));
+                else mbar_arrive(smem_u32(bar));
+            }
+        };
+        // a value tile with rows that were not loaded goes through the clearing warp while its scores are in softmax
+        auto ask_v = [&](int t, int v_it) {
+            if (!w.dirty(t)) return true;
+            if (!wait(&hdr->full[v_it % Sh::SLOTS], v_it / Sh::SLOTS, DEV_TIMEOUT_FULL)) return false;
+            if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ask));
+            ++n_v;
+            return true;
+        };
+        while (ok && w.next()) {
+            if (w.t0 >= w.t1) continue;
+            active = i == 0 || w.tok1 - w.tok0 > tpt;
+            int sl = it % Sh::SLOTS;
+            if (!wait(&hdr->q_full, q_no, DEV_TIMEOUT_FULL) || !wait(&hdr->full[sl], it / Sh::SLOTS, DEV_TIMEOUT_FULL)) break;
+            ++q_no;
+            tc_fence_after();
+            if (active && lane == 0) mma_s(sl);
+            release(&hdr->empty[sl]);
+            if (w.t0 + 1 == w.t1) release(&hdr->q_empty);
+            ++it;
+            ok = ask_v(w.t0, it);
+            for (int t = w.t0; t < w.t1 && ok; ++t) {
+                const int vs = it % Sh::SLOTS, ks = (it + 1) % Sh::SLOTS;
+                const bool more = t + 1 < w.t1;
+                ok = wait(&hdr->full[vs], it / Sh::SLOTS, DEV_TIMEOUT_FULL);
+                if (ok && w.dirty(t)) ok = wait(&hdr->v_ok, n_v - 1, DEV_TIMEOUT_FULL);
+                if (ok && more) ok = wait(&hdr->full[ks], (it + 1) / Sh::SLOTS, DEV_TIMEOUT_FULL);
+                if (ok && active) {
+                    ok = wait(&hdr->p_part[i], n_p, DEV_TIMEOUT_MMA);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) mma_o(vs, 4, 8, t > w.t0);
+                    ok = wait(&hdr->p_full[i], n_p, DEV_TIMEOUT_MMA);
+                    if (!ok) break;
+                    ++n_p;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        mma_o(vs, 0, 4, true);
+                        if (more) mma_s(ks);
                         else umma_commit(smem_u32(&hdr->o_full[i]));
                     }
-                    if (!ok) break;
-                    umma_commit(smem_u32(&hdr->empty[vs]));
-                    if (more) {
-                        umma_commit(smem_u32(&hdr->empty[ks]));
-                        if (t + 2 == w.t1) umma_commit(smem_u32(&hdr->q_empty));
-                    }
-                    it += more ? 2 : 1;
-                    if (more) ok = ask_v(t + 1, it);
                 }
+                if (!ok) break;
+                release(&hdr->empty[vs]);
+                if (more) {
+                    release(&hdr->empty[ks]);
+                    if (t + 2 == w.t1) release(&hdr->q_empty);
+                }
+                it += more ? 2 : 1;
+                if (more) ok = ask_v(t + 1, it);
             }
-            if (*cta_abort) {  // what was issued retires before the tensor memory is freed
-                umma_commit(smem_u32(&hdr->drain));
+        }
+        __syncwarp();
+        if (*cta_abort) {  // what was issued retires before the tensor memory is freed
+            if (lane == 0) {
+                umma_commit(smem_u32(&hdr->drain[i]));
                 const long long c0 = clock64();
-                while (!mbar_try_wait(smem_u32(&hdr->drain), 0))
+                while (!mbar_try_wait(smem_u32(&hdr->drain[i]), 0))
                     if (clock64() - c0 > WAIT_LIMIT_CYCLES) {
                         raise_status(DEV_TIMEOUT_DRAIN);
                         break;
                     }
             }
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (warp >= 10) {
-        // ------------------------------------------------------------ value tiles with keys that some row does not see
-        // Values that no row sees become zeros; where some row does not see a key, a value that is not finite does too (the
-        // tensor cores would add 0 * it), and the segment's rows are computed again by attn_row_exact.
-        // The issuing thread asks for each such tile when it has landed and waits for it before it asks for the next: these
-        // warps do not follow the ring's own barriers, most of whose phases they would skip.
+    } else if (warp == AT_WARP_CLEAR) {
+        // ------------------------------------------------------------ value tiles with rows that were not loaded
+        // Those become zeros (the tensor cores would add 0 * whatever was there).  The issuers ask for each such tile when it has
+        // landed and wait for it before they ask for the next: this warp does not follow the ring's own barriers, most of whose
+        // phases it would skip.
         int it = 0;
         uint32_t n_v = 0;
         bool ok = true;
         while (ok && w.next()) {
             for (int t = w.t0; t < w.t1; ++t, it += 2) {
-                if (!w.masked(t)) continue;
+                if (!w.dirty(t)) continue;
                 const int sl = (it + 1) % Sh::SLOTS;
                 if (!wait(&hdr->v_ask, n_v++, DEV_TIMEOUT_FULL)) {
                     ok = false;
                     break;
                 }
                 uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)(2 + sl) * Sh::TILE_BYTES);
-                const int k0 = t * AT_TILE;
-                bool odd = false;
-                for (int i = tid - 320; i < Sh::NCH * AT_TILE * 8; i += 64) {
-                    const int key = k0 + ((i >> 3) % AT_TILE);
-                    if (key >= w.kr.a2 && key < w.kr.b2) continue;
-                    bool clear = key < w.kr.a || key >= w.kr.b;
-                    if (!clear) {
-                        const uint4 y = vp[i];
-                        clear = has_nonfinite<T>(y.x) || has_nonfinite<T>(y.y) || has_nonfinite<T>(y.z) || has_nonfinite<T>(y.w);
-                        odd |= clear;
-                    }
-                    if (clear) vp[i] = make_uint4(0u, 0u, 0u, 0u);
+                const int c0 = min(max(((w.kr.a >> p.box_shift) << p.box_shift) - t * AT_TILE, 0), AT_TILE), c1 = max(min(w.si.kv - t * AT_TILE, AT_TILE), c0);
+                for (int ch = 0; ch < Sh::NCH; ++ch) {
+                    for (int i = lane; i < c0 * 8; i += 32) vp[ch * AT_TILE * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
+                    for (int i = c1 * 8 + lane; i < AT_TILE * 8; i += 32) vp[ch * AT_TILE * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
                 }
-                if (odd) *reinterpret_cast<volatile int*>(&hdr->nonfinite) = 1;  // (stays set: later segments of the CTA go the exact way too)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read by the tensor cores, refilled by a copy
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ok));
             }
         }
     } else {
-        // ------------------------------------------------------------ softmax and epilogue: a thread per row
-        const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        // ------------------------------------------------------------ softmax and epilogue: 16 rows per warp
+        const int wg = warp >> 3, row0 = (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + (lane >> 2);  // this lane's rows: row0, row0 + 8
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32 + ((warp >> 2) & 1) * 16) << 16;
         const uint32_t ts = tmem + lanes + AT_COL_S + 128u * wg, to = tmem + lanes + AT_COL_O + 128u * wg;
-        uint32_t n_s = 0, n_o = 0;
+        uint32_t n_s = 0, n_o = 0, n_turn = 0;
         const float c = p.scale_log2;
-        const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && (p.out_stride * (p.out_dtype == QMM_DT_F32 ? 4 : 2)) % 16 == 0;
         bool ok = true;
         while (ok && w.next()) {
-            const int n_tok = w.tok1 - w.tok0, tok = w.tok0 + wg * tpt + row / p.group;
-            if (wg * tpt >= n_tok) continue;  // no rows in this row tile
-            const bool live = row < tile_rows && tok < w.tok1;
-            const int pos = w.si.kv - w.si.q_len + tok;
-            const int hi = live ? max(pos + 1, 0) : 0, lo = p.window ? max(0, pos - p.window + 1) : 0;
-            float m = -INFINITY, l = 0.f;
+            const int n_tok = w.tok1 - w.tok0;
+            const bool both = n_tok > tpt;
+            if (wg == 1 && !both) continue;  // no rows in this row tile
+            int lo[2], hi[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int tok = w.tok0 + wg * tpt + ((row0 + 8 * e) * p.group_inv >> 16), pos = w.si.kv - w.si.q_len + tok;
+                hi[e] = row0 + 8 * e < tile_rows && tok < w.tok1 ? max(pos + 1, 0) : 0;
+                lo[e] = p.window ? max(0, pos - p.window + 1) : 0;
+            }
+            float m[2] = {-INFINITY, -INFINITY};
+            uint64_t l2[2] = {0ull, 0ull};  // sums of this lane's even and odd columns
             for (int t = w.t0; t < w.t1; ++t) {
                 if (!wait(&hdr->s_full[wg], n_s, DEV_TIMEOUT_MMA)) {
                     ok = false;
@@ -406,56 +588,69 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 }
                 ++n_s;
                 tc_fence_after();
-                uint32_t sr[4][32];  // the row
-#pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, sr[q]);
-                if (w.masked(t)) {
-                    const int k0 = t * AT_TILE;
-#pragma unroll
-                    for (int j = 0; j < AT_TILE; ++j)
-                        if (k0 + j < lo || k0 + j >= hi) sr[j >> 5][j & 31] = 0xFF800000u;  // -inf
-                }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int j = 0; j < AT_TILE; j += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[j >> 5][(j & 31) + 2 * e]), __uint_as_float(sr[j >> 5][(j & 31) + 2 * e + 1]));
-                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                if (t == w.t0) {
-                    m = mt;
-                } else {
-                    const bool grew = (mt - m) * c > 8.f || (m == -INFINITY && mt > -INFINITY);
-                    if (__any_sync(0xffffffffu, grew)) {
-                        const float mn = fmaxf(m, mt), f = mn == -INFINITY ? 1.f : fast_exp2((m - mn) * c);
-                        m = mn, l *= f;
+                // The rows' maxima from both halves of the keys; the second half stays in registers, the first is read again for
+                // its exponentials
+                const bool right = t >= w.u1, left = t < w.u0;
+                uint32_t sr[32];
+                float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-                        for (int q = 0; q < HD / 32; ++q) {
-                            uint32_t r[32];
-                            tmem_ld32(to + 32 * q, r);
+                for (int h = 0; h < 2; ++h) {
+                    tmem_ld_8(ts + 64 * h, sr);
+                    if (right) mask_right(sr, t * AT_TILE + 64 * h, hi);
+                    if (left) mask_left(sr, t * AT_TILE + 64 * h, lo);
+                    max64(sr, mt);
+                }
+                bool grew = false;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
-                            tmem_st32(to + 32 * q, r);
-                        }
+                for (int e = 0; e < 2; ++e) {
+                    mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 1));
+                    mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 2));
+                    grew |= (mt[e] - m[e]) * c > 8.f || (m[e] == -INFINITY && mt[e] > -INFINITY);
+                }
+                if (t == w.t0) {
+                    m[0] = mt[0], m[1] = mt[1];
+                } else if (__any_sync(0xffffffffu, grew)) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float mn = fmaxf(m[e], mt[e]);
+                        f[e] = mn == -INFINITY ? 1.f : fast_exp2((m[e] - mn) * c);
+                        m[e] = mn, l2[e] = mul2(l2[e], f32x2(f[e], f[e]));
+                    }
+#pragma unroll 1
+                    for (int q = 0; q < HD / 32; ++q) {
+                        uint32_t r[16];
+                        tmem_ld_4(to + 32 * q, r);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f[(j >> 1) & 1]);
+                        tmem_st_4(to + 32 * q, r);
                     }
                 }
-                const float mc = m == -INFINITY ? 0.f : m * c;
-                float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float e0 = fast_exp2(fmaf(__uint_as_float(sr[q][2 * j]), c, -mc)), e1 = fast_exp2(fmaf(__uint_as_float(sr[q][2 * j + 1]), c, -mc));
-                        ls[j & 1] += e0, ls[2 + (j & 1)] += e1;
-                        pk[j] = pack2<T>(e0, e1);
+                // The two row tiles take turns at the exponentials: left to themselves both wait for scores at the same time and then
+                // share the special-function units, while the tensor cores idle (8192 tokens, 32/8 heads: 619 us without turns, 550 with;
+                // per scheduler, warp & 3: whoever is ready there goes on)
+                if (both) {
+                    if ((wg == 1 || n_turn > 0) && !wait(&hdr->turn[wg][warp & 3], wg == 1 ? n_turn : n_turn - 1, DEV_TIMEOUT_MMA)) {
+                        ok = false;
+                        break;
                     }
-                    tmem_st16(ts + 16 * q, pk);
+                    ++n_turn;
                 }
-                l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&hdr->p_full[wg]));
+                const float mc[2] = {m[0] == -INFINITY ? 0.f : m[0] * c, m[1] == -INFINITY ? 0.f : m[1] * c};
+#pragma unroll 1
+                for (int h = 1; h >= 0; --h) {  // the second half, in registers, first
+                    if (h == 0) {
+                        tmem_ld_8(ts, sr);
+                        if (right) mask_right(sr, t * AT_TILE, hi);
+                        if (left) mask_left(sr, t * AT_TILE, lo);
+                    }
+                    exp64<T>(sr, c, mc, ts + AT_COL_P + 32 * h, l2);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(h ? &hdr->p_part[wg] : &hdr->p_full[wg]));  // the product of this half can begin
+                }
+                if (both && lane == 0) mbar_arrive(smem_u32(&hdr->turn[wg ^ 1][warp & 3]));
             }
             if (!ok) break;
             if (w.t0 < w.t1) {
@@ -464,76 +659,77 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 tc_fence_after();
             }
             const bool whole = w.begins && w.ends;
-            const int slot = 2 * (int)blockIdx.x + (w.begins ? 1 : 0), r = (tok - w.tok0) * p.group + row % p.group;  // row of the item
-            const int head = w.kvh * p.group + row % p.group;
+            const int slot = 2 * (int)blockIdx.x + (w.begins ? 1 : 0);
             float* ml = whole ? nullptr : ArScratch<HD, AT_MAX_ROWS>::ml(p.scratch, gridDim.x, slot);
             float* so = whole ? nullptr : ArScratch<HD, AT_MAX_ROWS>::o(p.scratch, gridDim.x, slot);
-            const size_t oe = (size_t)(w.si.q0 + tok) * p.out_stride + (size_t)head * HD;
-            if (*reinterpret_cast<volatile int*>(&hdr->nonfinite)) {
-                // a row at a time by the whole warp
-                for (int u = 0; u < 32; ++u) {
-                    const int rr = (warp & 3) * 32 + u, tk = w.tok0 + wg * tpt + rr / p.group, ps = w.si.kv - w.si.q_len + tk, hd = w.kvh * p.group + rr % p.group;
-                    if (rr >= tile_rows || tk >= w.tok1) break;
-                    float em, el, eo[HD / 32];
-                    attn_row_exact<T, HD>(p, w.s, w.si.q0, tk, hd, w.kvh, max(w.st0 * AT_TILE, p.window ? max(0, ps - p.window + 1) : 0),
-                                          min(w.st1 * AT_TILE, ps + 1), em, el, eo);
-                    const int r2 = (tk - w.tok0) * p.group + rr % p.group;
-                    const float inv = 1.f / el;
+            {
+                // f32 (and what is joined later): 8 bytes per lane, 32-byte pieces; 16-bit outputs of 32 columns are turned within
+                // the four lanes of a row, 16 bytes per lane, 64-byte pieces
+                const bool f32 = !whole || p.out_dtype == QMM_DT_F32;
+                const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % 8 == 0;
+                char* dst[2];
+                float inv[2];
+                bool live[2], sees[2];
 #pragma unroll
-                    for (int j = 0; j < HD / 32; ++j) {
-                        if (whole) store_out1(p.out, p.out_dtype, (size_t)(w.si.q0 + tk) * p.out_stride + (size_t)hd * HD + lane + 32 * j, ps >= 0 ? eo[j] * inv : 0.f);
-                        else so[(size_t)r2 * HD + lane + 32 * j] = eo[j];
-                    }
-                    if (!whole && lane == 0) ml[2 * r2] = em, ml[2 * r2 + 1] = el;
+                for (int e = 0; e < 2; ++e) {
+                    const int row = row0 + 8 * e, tk = row * p.group_inv >> 16, g = row - tk * p.group, tok = w.tok0 + wg * tpt + tk;
+                    float l = lo2(l2[e]) + hi2(l2[e]);
+                    l += __shfl_xor_sync(0xffffffffu, l, 1);
+                    l += __shfl_xor_sync(0xffffffffu, l, 2);
+                    live[e] = row < tile_rows && tok < w.tok1, sees[e] = w.si.kv - w.si.q_len + tok >= 0;
+                    inv[e] = whole ? 1.f / l : 1.f;
+                    const int r = (tok - w.tok0) * p.group + g;  // row of the item
+                    const size_t oe = (size_t)(w.si.q0 + tok) * p.out_stride + (size_t)(w.kvh * p.group + g) * HD;
+                    dst[e] = whole ? static_cast<char*>(p.out) + oe * (f32 ? 4 : 2) : reinterpret_cast<char*>(so + (size_t)r * HD);
+                    if (!whole && live[e] && (lane & 3) == 0) ml[2 * r] = m[e], ml[2 * r + 1] = l;
                 }
-            } else {
-                const bool sees = pos >= 0;
-                const float inv = 1.f / l;
-#pragma unroll 1
+                float odd[2] = {0.f, 0.f};
+#pragma unroll 2
                 for (int q = 0; q < HD / 32; ++q) {
-                    uint32_t o[32];
+                    uint32_t o[16];
                     if (w.t0 < w.t1) {
-                        tmem_ld32(to + 32 * q, o);
+                        tmem_ld_4(to + 32 * q, o);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = 0u;
+                        for (int j = 0; j < 16; ++j) o[j] = 0u;
                     }
-                    if (live) {
-                        if (!whole) {
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4)
-                                *reinterpret_cast<uint4*>(so + (size_t)r * HD + 32 * q + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    for (int j = 0; j < 16; ++j) odd[(j >> 1) & 1] += __uint_as_float(o[j]) * 0.f;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = whole && !sees[e] ? 0.f : __uint_as_float(o[4 * (j >> 1) + 2 * e + (j & 1)]) * inv[e];
+                        if (f32) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (live[e]) *reinterpret_cast<float2*>(dst[e] + (32 * q + 8 * i + 2 * (lane & 3)) * 4) = make_float2(v[2 * i], v[2 * i + 1]);
                         } else {
+                            uint32_t h[4];
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = sees ? __float_as_uint(__uint_as_float(o[j]) * inv) : 0u;
-                            if (vec && p.out_dtype == QMM_DT_F32) {
+                            for (int i = 0; i < 4; ++i)
+                                h[i] = p.out_dtype == QMM_DT_F16 ? pack2<__half>(v[2 * i], v[2 * i + 1]) : pack2<__nv_bfloat16>(v[2 * i], v[2 * i + 1]);
+                            if (vec) {
+                                turn4(h);
+                                if (live[e]) *reinterpret_cast<uint4*>(dst[e] + (32 * q + 8 * (lane & 3)) * 2) = make_uint4(h[0], h[1], h[2], h[3]);
+                            } else if (live[e]) {
 #pragma unroll
-                                for (int j = 0; j < 32; j += 4)
-                                    *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + oe + 32 * q + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                            } else if (vec) {
-                                uint32_t h[16];
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) {
-                                    const float a = __uint_as_float(o[2 * j]), b = __uint_as_float(o[2 * j + 1]);
-                                    h[j] = p.out_dtype == QMM_DT_F16 ? pack2<__half>(a, b) : pack2<__nv_bfloat16>(a, b);
-                                }
-#pragma unroll
-                                for (int j = 0; j < 16; j += 4)
-                                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + oe + 32 * q + 2 * j) = make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 32; j += 2) store_out2(p.out, p.out_dtype, oe + 32 * q + j, __uint_as_float(o[j]), __uint_as_float(o[j + 1]));
+                                for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(dst[e] + (32 * q + 8 * i + 2 * (lane & 3)) * 2) = h[i];
                             }
                         }
                     }
                 }
-                if (!whole && live) ml[2 * r] = m, ml[2 * r + 1] = l;
+                // outputs that are not finite: from a value that the row does not see, or by the formula; either way again, exactly
+                if (__any_sync(0xffffffffu, (live[0] && odd[0] != odd[0]) || (live[1] && odd[1] != odd[1])))
+                    at_exact_rows<T, HD>(p, w, wg * tpt, row0 - (lane >> 2), tile_rows, whole, so, ml);
             }
             if (w.begins && !w.ends && tid == 0) {  // this item goes on in the next CTAs: how many of them
                 ArJoin j;
                 j.s = w.s, j.q0 = w.si.q0, j.tok_row0 = w.tok0 * p.group, j.n_rows = n_tok * p.group, j.kvh = w.kvh;
                 j.any_key = w.si.kv - w.si.q_len;
-                const long item_end = w.g1 + (w.nt - (w.st1 - w.tl));
+                const long total = hdr->scan[34];
+                const int n_ctas = (int)hdr->scan[35];
+                const long item_end = ar_share(total, blockIdx.x + 1, n_ctas) + (w.nt - (w.st1 - w.tl));
                 int e = blockIdx.x + 1;
                 while (ar_share(total, e + 1, n_ctas) < item_end) ++e;
                 j.n_parts = e - (int)blockIdx.x + 1, j.pad = 0;
@@ -543,7 +739,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == AT_WARP_MMA0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -565,9 +761,10 @@ static int attn_tiles_inst(const AttnParams& p, const CUtensorMap& qm, const CUt
         }
     }
     const int tb = 2 * (AT_TILE / p.group), ctas = sm_count();
-    const long blocks = (long)p.total_q / tb + p.n_seqs;  // at least as many as there are
-    if (!p.stream_k && blocks > 65535) return QMM_ERR_UNSUPPORTED;
-    if (int st = launch_overlapped(attn_tiles_kernel<T, HD>, p.stream_k ? dim3(ctas) : dim3(p.nkv, (unsigned)blocks), dim3(AT_THREADS), smem, s, qm, km, vm, p)) return st;
+    const long items = ((long)p.total_q / tb + p.n_seqs) * p.nkv;  // at least as many as there are
+    if (items > 1l << 30) return QMM_ERR_UNSUPPORTED;
+    const int grid = p.stream_k ? ctas : (int)(items < ctas ? items : ctas);
+    if (int st = launch_overlapped(attn_tiles_kernel<T, HD>, dim3(grid), dim3(AT_THREADS), smem, s, qm, km, vm, p)) return st;
     if (p.stream_k) return launch_overlapped(attn_join_kernel<HD, AT_MAX_ROWS>, dim3(ctas, AT_MAX_ROWS / 4), dim3(128), 0, s, p, ctas);
     return QMM_OK;
 }
