@@ -42,9 +42,17 @@ __device__ __forceinline__ void raise_status(int code) { atomicExch(&g_device_st
 
 // A bounded wait whose first probe alone is inlined: these kernels wait in many places, and their code has to fit the
 // instruction cache (items of a few tiles spent most of their time fetching code when everything was inlined and unrolled).
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* cta_abort) { return mbar_wait_bounded(bar, parity, cta_abort); }
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* cta_abort) {
-    return mbar_try_wait(smem_u32(bar), parity) || wait_slow(smem_u32(bar), parity, cta_abort);
+// Where the wait runs out the CTA's abort flag is set and the status raised.
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, int code, volatile int* cta_abort) {
+    if (mbar_wait_bounded(bar, parity, cta_abort)) return true;
+    if (!*cta_abort) {
+        raise_status(code);
+        *cta_abort = 1;
+    }
+    return false;
+}
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int code, volatile int* cta_abort) {
+    return mbar_try_wait(smem_u32(bar), parity) || wait_slow(smem_u32(bar), parity, code, cta_abort);
 }
 
 // The lengths of a sequence, held inside the buffers whatever the arrays say (a value outside raises the device status).
@@ -92,10 +100,11 @@ __device__ __forceinline__ int page_of(const AttnParams& p, int s, int page_idx)
     return id;
 }
 
-// Block-wide search: f(s) >= 0 items per sequence; finds the sequence that holds item `target` of all of them and the items
+// Block-wide search: F::count(p, s) >= 0 items per sequence; finds the sequence that holds item `target` of all of them and the items
 // before it.  Every thread of the block calls it; sh: 36 words.  Returns -1 when there are fewer items (total in `before`).
 template <typename F>
-__device__ __forceinline__ int find_item(int n_seqs, long target, F f, long& before, long long* sh) {
+__device__ __noinline__ int find_item(const AttnParams& p, long target, long& before, long long* sh) {
+    const int n_seqs = p.n_seqs;
     const int nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = nt >> 5;
     long base = 0;
     int found = -1;
@@ -103,7 +112,7 @@ __device__ __forceinline__ int find_item(int n_seqs, long target, F f, long& bef
 #pragma unroll 1
     for (int s0 = 0; s0 < n_seqs; s0 += nt) {
         const int s = s0 + threadIdx.x;
-        const long long v = s < n_seqs ? (long long)f(s) : 0ll;
+        const long long v = s < n_seqs ? (long long)F::count(p, s) : 0ll;
         long long inc = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {

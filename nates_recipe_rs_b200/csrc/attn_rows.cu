@@ -96,11 +96,6 @@ struct ArWalker {
         nt = max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - tl);
         nrb = (si.q_len * p.group + R - 1) / R;
     }
-    __device__ static __forceinline__ long tiles_of(const AttnParams& p, int s) {
-        const SeqInfo si = seq_info(p, s);
-        const KeyRange kr = key_range(p, si, 0, si.q_len);
-        return (long)((si.q_len * p.group + R - 1) / R) * p.nkv * max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - kr.a / AR_TILE);
-    }
     __device__ __noinline__ bool next() {
         if (g >= g1) return false;
         while (item >= nrb * p.nkv) {  // (sequences without rows have no items)
@@ -116,6 +111,16 @@ struct ArWalker {
         if (within == nt) within = 0, ++item;
         return true;
     }
+};
+template <int R> struct ArTiles {  // tiles of all items of a sequence
+    __device__ static __forceinline__ long count(const AttnParams& p, int s) {
+        const SeqInfo si = seq_info(p, s);
+        const KeyRange kr = key_range(p, si, 0, si.q_len);
+        return (long)((si.q_len * p.group + R - 1) / R) * p.nkv * max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - kr.a / AR_TILE);
+    }
+};
+template <int R> struct ArBlocks {  // row blocks of a sequence
+    __device__ static __forceinline__ long count(const AttnParams& p, int s) { return (seq_info(p, s).q_len * p.group + R - 1) / R; }
 };
 // First tile of CTA c of n when `total` tiles are shared evenly
 __device__ __noinline__ long ar_share(long total, int c, int n) { return total * c / n; }
@@ -161,20 +166,20 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
     if (p.stream_k) {
         // all tiles, then the sequence this CTA's share starts in
         long before = 0;
-        find_item(p.n_seqs, 1l << 62, [&](int s) { return ArWalker<R>::tiles_of(p, s); }, total, hdr->scan);
+        find_item<ArTiles<R>>(p, 1l << 62, total, hdr->scan);
         n_ctas = ar_ctas(total, gridDim.x);
         ArJoin* join = reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x;
         if (tid == 0) join->n_rows = 0;
         if ((int)blockIdx.x >= n_ctas) return;
         w.g = ar_share(total, blockIdx.x, n_ctas), w.g1 = ar_share(total, blockIdx.x + 1, n_ctas);
-        w.s = find_item(p.n_seqs, w.g, [&](int s) { return ArWalker<R>::tiles_of(p, s); }, before, hdr->scan);
+        w.s = find_item<ArTiles<R>>(p, w.g, before, hdr->scan);
         if (w.s < 0) return;  // (no rows at all)
         w.load_seq();
         w.item = (int)((w.g - before) / w.nt), w.within = (int)((w.g - before) % w.nt);
     } else {
         // one item per CTA: block row blockIdx.y of all row blocks (a sequence's last, longest, first), kv head blockIdx.x
         long before = 0;
-        w.s = find_item(p.n_seqs, blockIdx.y, [&](int s) { return ((long)seq_info(p, s).q_len * p.group + R - 1) / R; }, before, hdr->scan);
+        w.s = find_item<ArBlocks<R>>(p, blockIdx.y, before, hdr->scan);
         if (w.s < 0) return;
         w.load_seq();
         w.g = 0, w.g1 = w.nt, w.within = 0;
@@ -183,12 +188,6 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
     __syncthreads();
     int it = 0;  // tiles so far, over all segments: stage it % STAGES
 
-    auto give_up = [&](int code) {
-        if (!*cta_abort) {
-            raise_status(code);
-            *cta_abort = 1;
-        }
-    };
     // the tokens of a row block, and the tiles of a segment that hold keys of its rows
     auto block_range = [&](int& tok0, int& n_rows, KeyRange& kr, int& t0, int& t1) {
         const int r0 = w.rb * R;
@@ -216,10 +215,7 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
                     tile_boxes<AR_TILE>(p, t + 1, kr.a, w.si.kv, nfirst, ncount);
                     npages = page_of_boxes<AR_TILE>(p, w.s, w.si.q0, t + 1, nfirst, ncount, nslots);
                 }
-                if (it >= Sh::STAGES && !wait_bar(&hdr->empty[st], ((it / Sh::STAGES) - 1) & 1, cta_abort)) {
-                    if (lane == 0) give_up(DEV_TIMEOUT_EMPTY);
-                    break;
-                }
+                if (it >= Sh::STAGES && !wait_bar(&hdr->empty[st], ((it / Sh::STAGES) - 1) & 1, DEV_TIMEOUT_EMPTY, cta_abort)) break;
                 const uint32_t bar = smem_u32(&hdr->full[st]), dst = ring + (uint32_t)st * 2 * Sh::TILE_BYTES;
                 if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(count * 2 * Sh::NCH * 128) << p.box_shift);
                 __syncwarp();
@@ -284,9 +280,7 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
 
         for (int t = t0; t < t1; ++t, ++it) {
             const int st = it % Sh::STAGES;
-            if (!wait_bar(&hdr->full[st], (it / Sh::STAGES) & 1, cta_abort)) {
-                if (lane == 0) give_up(DEV_TIMEOUT_FULL);  // (on to the end all the same: the warps meet at barriers)
-            }
+            wait_bar(&hdr->full[st], (it / Sh::STAGES) & 1, DEV_TIMEOUT_FULL, cta_abort);  // (on to the end even if it runs out: the warps meet at barriers)
             const uint32_t ks = ring + (uint32_t)st * 2 * Sh::TILE_BYTES, vs = ks + Sh::TILE_BYTES;
             const int k0 = t * AR_TILE;
             const bool masked = k0 < kr.a2 || k0 + AR_TILE > kr.b2;  // some row does not see some key of the tile

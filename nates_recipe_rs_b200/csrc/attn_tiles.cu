@@ -16,7 +16,9 @@
 // warps per tile, a warp had no one to share its scheduler with and issued every third cycle; 16 and 19 issue the tcgen05.mma of
 // row tile 0 / 1 (an issuing thread blocks while the tensor cores are busy, and every wait or commit costs it some 90 cycles more:
 // with one issuer for both tiles these were idle time of the tensor cores); 17 issues the TMA copies (queries, and keys and values
-// through a ring of 128-key slots); 18 clears what no row sees out of the value tiles that need it.
+// through a ring of 128-key slots); 18 plans: it alone works out which item comes next and hands the others its bounds through
+// shared memory, ahead of time (done by every warp for itself this took each some 4000 cycles per item), and it clears what was not
+// loaded out of the value tiles that need it.
 // The CTAs stay: each takes items until none is left, so that the copies and the scores of the next item run under the epilogue
 // of the one before (a CTA per item spent 7 us between the last tile of one and the first of the next).
 // Every wait is bounded; on expiry the CTA records a status code, drains its copies, frees its tensor memory and returns.
@@ -25,8 +27,10 @@
 namespace qmm {
 
 constexpr int AT_TILE = 128;  // keys per tile, and rows per tile
-constexpr int AT_THREADS = 640;  // 16 softmax warps, two issuing warps, the copying and the clearing warp
-constexpr int AT_WARP_MMA0 = 16, AT_WARP_COPY = 17, AT_WARP_CLEAR = 18, AT_WARP_MMA1 = 19;
+constexpr int AT_THREADS = 640;  // 16 softmax warps, two issuing warps, the copying and the planning warp (a 21st would leave 80 registers)
+constexpr int AT_WARP_MMA0 = 16, AT_WARP_COPY = 17, AT_WARP_PLAN = 18, AT_WARP_MMA1 = 19;
+constexpr int AT_SEGS = 4;  // segments planned ahead
+constexpr int AT_FEW_SEQS = 64;  // up to this many sequences the planning warp finds its place alone, beyond the whole CTA does
 constexpr int AT_MAX_ROWS = 256;  // rows of an item
 template <int HD> struct AtShape {
     static constexpr int NCH = (HD + 63) / 64;
@@ -39,8 +43,26 @@ template <int HD> struct AtShape {
 // tile i at 256 + 128 i
 constexpr uint32_t AT_COL_S = 0, AT_COL_P = 64, AT_COL_O = 256;
 
+// A segment: some of the key tiles of an item, as the planning warp hands it to the others
+struct AtSeg {
+    int valid;          // 0: no more
+    int s, q0, q_len, kv;
+    int kvh, tok0, tok1;  // tokens [tok0, tok1) of the sequence
+    int t0, t1;         // tiles [t0, t1) that hold keys of its rows
+    int st0, st1;       // tiles of the segment before that cut
+    int u0, u1;         // tiles [u0, u1) whose keys every row sees
+    int d0, d1;         // tiles [d0, d1) that are loaded whole
+    int a;              // first key that any row sees
+    int begins, ends;   // the item's first / last segment
+    int more;           // tiles of the item after the segment
+
+    // rows of value tile t were not loaded, or are not of this sequence
+    __device__ __forceinline__ bool dirty(int t) const { return t < d0 || t >= d1; }
+};
+
 struct __align__(16) AtHeader {
-    uint64_t full[10], empty[10];
+    uint64_t full[10], empty[10], seg_full[AT_SEGS], seg_empty[AT_SEGS];
+    AtSeg seg[AT_SEGS];
     uint64_t v_ask, v_ok, q_full, q_empty, s_full[2], p_part[2], p_full[2], o_full[2], turn[2][4], drain[2];
     long long scan[36];
     AttnParams p;  // a copy: functions that are not inlined would fetch the kernel's parameters from far away, one by one
@@ -160,23 +182,44 @@ __device__ __forceinline__ void exp64(const uint32_t (&s)[32], float c, const fl
     tmem_st_p(tp, pk);
 }
 
-// Four words per lane in four lanes: afterwards lane j of the four holds word j of every lane, in lane order
-__device__ __forceinline__ void turn4(uint32_t (&v)[4]) {
-#pragma unroll
-    for (int d = 1; d <= 2; d <<= 1) {
-        const bool up = threadIdx.x & d;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (k & d) continue;
-            const uint32_t x = __shfl_xor_sync(0xffffffffu, up ? v[k] : v[k + d], d);
-            if (up) v[k] = x;
-            else v[k + d] = x;
-        }
+__device__ __forceinline__ int at_block_tokens(const AttnParams& p) { return 2 * (AT_TILE * p.group_inv >> 16); }  // of an item
+__device__ __forceinline__ int at_tile_count(const KeyRange& kr) { return max(1, (max(kr.b, 0) + AT_TILE - 1) / AT_TILE - kr.a / AT_TILE); }
+struct AtItems {  // items of a sequence
+    __device__ static __forceinline__ int count(const AttnParams& p, int s) { return (seq_info(p, s).q_len + at_block_tokens(p) - 1) / at_block_tokens(p) * p.nkv; }
+};
+struct AtTiles {  // tiles of them all
+    __device__ static __forceinline__ long count(const AttnParams& p, int s) {
+        const SeqInfo si = seq_info(p, s);
+        return (long)((si.q_len + at_block_tokens(p) - 1) / at_block_tokens(p)) * p.nkv * at_tile_count(key_range(p, si, 0, si.q_len));
     }
+};
+
+// As find_item, by one warp: 32 sequences at a time
+template <typename F>
+__device__ __noinline__ int warp_find_item(const AttnParams& p, long target, long& before) {
+    const int lane = threadIdx.x & 31;
+    before = 0;
+#pragma unroll 1
+    for (int base = 0; base < p.n_seqs; base += 32) {
+        const long long cnt = base + lane < p.n_seqs ? (long long)F::count(p, base + lane) : 0ll;
+        long long inc = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + inc > target);
+        if (past) {
+            const int f = __ffs(past) - 1;
+            before += __shfl_sync(0xffffffffu, inc - cnt, f);
+            return base + f;
+        }
+        before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return -1;
 }
 
-// The segments (item, tiles [t0, t1) of it) of this CTA; every warp of the CTA walks them (whole warps, all lanes alike).  An item
-// is (sequence, kv head, block of tb tokens).
+// The segments of this CTA, walked by the planning warp.  An item is (sequence, kv head, block of tb tokens).
 // Many items: whole items, CTA c of n takes number c, 2n-1-c, 2n+c, ... of all (a sequence's last, longest blocks first, every
 // second round backwards: the rounds' differences cancel).  Few items over a long axis (stream_k): all tiles are shared evenly in
 // order, where every item of a sequence counts as many tiles as its last block has, at least one.
@@ -188,28 +231,13 @@ struct AtWalker {
     int s, item, within;
     SeqInfo si;
     int tl, nt, nb;
-    // the current segment
-    int kvh, tok0, tok1, t0, t1;  // tokens [tok0, tok1), tiles [t0, t1) that hold keys of its rows
-    int st0, st1;                 // tiles of the segment before that cut
-    int u0, u1;                   // tiles [u0, u1) whose keys every row sees
-    int d0, d1;                   // tiles [d0, d1) that are loaded whole
-    bool begins, ends;
-    KeyRange kr;
 
-    __device__ static __forceinline__ int count(const SeqInfo& si, const KeyRange& kr) {
-        return max(1, (max(kr.b, 0) + AT_TILE - 1) / AT_TILE - kr.a / AT_TILE);
-    }
     __device__ __forceinline__ void load_seq() {
         si = seq_info(p, s);
         const KeyRange r = key_range(p, si, 0, si.q_len);
         tl = r.a / AT_TILE;
-        nt = count(si, r);
+        nt = at_tile_count(r);
         nb = (si.q_len + tb - 1) / tb;
-    }
-    __device__ static __forceinline__ int items_of(const AttnParams& p, int tb, int s) { return (seq_info(p, s).q_len + tb - 1) / tb * p.nkv; }
-    __device__ static __forceinline__ long tiles_of(const AttnParams& p, int tb, int s) {
-        const SeqInfo si = seq_info(p, s);
-        return (long)((si.q_len + tb - 1) / tb) * p.nkv * count(si, key_range(p, si, 0, si.q_len));
     }
     // To the item `n` after the current one; 32 sequences are looked at at a time.
     __device__ __forceinline__ bool skip(int n) {
@@ -217,9 +245,10 @@ struct AtWalker {
         int target = item + n;
         if (target >= nb * p.nkv) {
             target -= nb * p.nkv;
+#pragma unroll 1
             for (int base = s + 1;; base += 32) {
                 if (base >= p.n_seqs) return false;
-                const int cnt = base + lane < p.n_seqs ? items_of(p, tb, base + lane) : 0;
+                const int cnt = base + lane < p.n_seqs ? AtItems::count(p, base + lane) : 0;
                 int inc = cnt;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -240,8 +269,7 @@ struct AtWalker {
         item = target;
         return true;
     }
-    // (not inlined: five roles call it, and code that runs once per item should not push the loops out of the instruction cache)
-    __device__ __noinline__ bool next() {
+    __device__ __forceinline__ bool next(AtSeg& g) {
         if (left <= 0) return false;
         int blk;
         if (p.stream_k) {
@@ -251,49 +279,47 @@ struct AtWalker {
                 load_seq();
             }
             const int n = min(left, nt - within);
-            kvh = item / nb, blk = item - kvh * nb;
-            st0 = tl + within, st1 = st0 + n;
-            begins = within == 0, ends = within + n == nt;
+            g.kvh = item / nb, blk = item - g.kvh * nb;
+            g.st0 = tl + within, g.st1 = g.st0 + n;
+            g.begins = within == 0, g.ends = within + n == nt;
             left -= n, within += n;
+            g.more = nt - within;
             if (within == nt) within = 0, ++item;
         } else {
-            if (!skip(ahead)) {
-                left = 0;
-                return false;
-            }
+            if (!skip(ahead)) return false;
             const int n = gridDim.x, c = blockIdx.x;
             ahead = (turn++ & 1) ? 2 * c + 1 : 2 * (n - c) - 1;
-            blk = item / p.nkv, kvh = item - blk * p.nkv, blk = nb - 1 - blk;
-            st0 = tl, st1 = tl + nt;
-            begins = ends = true;
+            blk = item / p.nkv, g.kvh = item - blk * p.nkv, blk = nb - 1 - blk;
+            g.st0 = tl, g.st1 = tl + nt;
+            g.begins = g.ends = 1, g.more = 0;
         }
-        tok0 = blk * tb, tok1 = min(tok0 + tb, si.q_len);
-        kr = key_range(p, si, tok0, tok1);
-        t0 = max(st0, kr.a / AT_TILE), t1 = min(st1, (kr.b + AT_TILE - 1) / AT_TILE);
-        u0 = (kr.a2 + AT_TILE - 1) / AT_TILE, u1 = kr.b2 / AT_TILE;
-        d0 = (((kr.a >> p.box_shift) << p.box_shift) + AT_TILE - 1) / AT_TILE, d1 = si.kv / AT_TILE;
+        g.valid = 1, g.s = s, g.q0 = si.q0, g.q_len = si.q_len, g.kv = si.kv;
+        g.tok0 = blk * tb, g.tok1 = min(g.tok0 + tb, si.q_len);
+        const KeyRange kr = key_range(p, si, g.tok0, g.tok1);
+        g.a = kr.a;
+        g.t0 = max(g.st0, kr.a / AT_TILE), g.t1 = min(g.st1, (kr.b + AT_TILE - 1) / AT_TILE);
+        g.u0 = (kr.a2 + AT_TILE - 1) / AT_TILE, g.u1 = kr.b2 / AT_TILE;
+        g.d0 = (((kr.a >> p.box_shift) << p.box_shift) + AT_TILE - 1) / AT_TILE, g.d1 = si.kv / AT_TILE;
         return true;
     }
-    // rows of value tile t were not loaded, or are not of this sequence
-    __device__ __forceinline__ bool dirty(int t) const { return t < d0 || t >= d1; }
 };
 
 // The 16 rows of a warp (rows row0 .. row0 + 15 of the row tile whose first token is tok0 of the block) without the tensor cores
 template <typename T, int HD>
-__device__ __noinline__ void at_exact_rows(const AttnParams& p, const AtWalker& w, int tok0, int row0, int tile_rows, bool whole, float* so, float* ml) {
+__device__ __noinline__ void at_exact_rows(const AttnParams& p, const AtSeg& w, int tok0, int row0, int tile_rows, bool whole, float* so, float* ml) {
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
     for (int row = row0; row < row0 + 16; ++row) {
-        const int tok = w.tok0 + tok0 + row / p.group, pos = w.si.kv - w.si.q_len + tok, head = w.kvh * p.group + row % p.group;
+        const int tok = w.tok0 + tok0 + row / p.group, pos = w.kv - w.q_len + tok, head = w.kvh * p.group + row % p.group;
         if (row >= tile_rows || tok >= w.tok1) break;
         float m, l, o[HD / 32];
-        attn_row_exact<T, HD>(p, w.s, w.si.q0, tok, head, w.kvh, max(w.st0 * AT_TILE, p.window ? max(0, pos - p.window + 1) : 0),
+        attn_row_exact<T, HD>(p, w.s, w.q0, tok, head, w.kvh, max(w.st0 * AT_TILE, p.window ? max(0, pos - p.window + 1) : 0),
                               min(w.st1 * AT_TILE, pos + 1), m, l, o);
         const int r = (tok - w.tok0) * p.group + row % p.group;
         const float inv = 1.f / l;
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
-            if (whole) store_out1(p.out, p.out_dtype, (size_t)(w.si.q0 + tok) * p.out_stride + (size_t)head * HD + lane + 32 * j, pos >= 0 ? o[j] * inv : 0.f);
+            if (whole) store_out1(p.out, p.out_dtype, (size_t)(w.q0 + tok) * p.out_stride + (size_t)head * HD + lane + 32 * j, pos >= 0 ? o[j] * inv : 0.f);
             else so[(size_t)r * HD + lane + 32 * j] = o[j];
         }
         if (!whole && lane == 0) ml[2 * r] = m, ml[2 * r + 1] = l;
@@ -318,6 +344,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         for (int i = 0; i < Sh::SLOTS; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), 2);
         mbar_init(smem_u32(&hdr->v_ask), 2), mbar_init(smem_u32(&hdr->v_ok), 1);
         mbar_init(smem_u32(&hdr->q_full), 1), mbar_init(smem_u32(&hdr->q_empty), 2);
+        for (int i = 0; i < AT_SEGS; ++i) mbar_init(smem_u32(&hdr->seg_full[i]), 1), mbar_init(smem_u32(&hdr->seg_empty[i]), 19);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&hdr->s_full[i]), 1), mbar_init(smem_u32(&hdr->o_full[i]), 1), mbar_init(smem_u32(&hdr->drain[i]), 1);
             mbar_init(smem_u32(&hdr->p_part[i]), 8), mbar_init(smem_u32(&hdr->p_full[i]), 8);
@@ -335,79 +362,133 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
     pdl_wait_prior_grids();
     pdl_release_dependents();
 
-    AtWalker w{p, 2 * tpt};
-    int n_ctas = 1;
-    long total = 0, before = 0;
-    bool any;
-    if (p.stream_k) {
-        find_item(p.n_seqs, 1l << 62, [&](int s) { return AtWalker::tiles_of(p, 2 * tpt, s); }, total, hdr->scan);
-        n_ctas = ar_ctas(total, gridDim.x);
-        if (tid == 0) (reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x)->n_rows = 0;
-        const long g = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
-        w.left = (int)(ar_share(total, min((int)blockIdx.x + 1, n_ctas), n_ctas) - g);
-        w.s = find_item(p.n_seqs, g, [&](int s) { return AtWalker::tiles_of(p, 2 * tpt, s); }, before, hdr->scan);
-        any = (int)blockIdx.x < n_ctas && w.s >= 0;
-        if (any) {
-            w.load_seq();
-            w.item = (int)((g - before) / w.nt), w.within = (int)((g - before) % w.nt);
-        }
-    } else {
-        // whole items: the first is number blockIdx.x (few sequences: the walk finds it by itself)
-        any = true;
-        w.s = -1, w.item = w.nb = w.within = 0, w.left = 1, w.ahead = blockIdx.x, w.turn = 0;
-        if (p.n_seqs > 64) {
-            w.s = find_item(p.n_seqs, blockIdx.x, [&](int s) { return AtWalker::items_of(p, 2 * tpt, s); }, before, hdr->scan);
-            any = w.s >= 0;
-            if (any) {
-                w.load_seq();
-                w.item = (int)(blockIdx.x - before), w.ahead = 0;
-            }
+    // many sequences: their lengths are read by all threads
+    long total = 0, before = 0, share = 0;
+    int first_seq = -1, n_ctas = 1;
+    if (p.n_seqs > AT_FEW_SEQS) {
+        if (p.stream_k) {
+            find_item<AtTiles>(p, 1l << 62, total, hdr->scan);
+            n_ctas = ar_ctas(total, gridDim.x), share = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
+            first_seq = find_item<AtTiles>(p, share, before, hdr->scan);
+        } else {
+            first_seq = find_item<AtItems>(p, blockIdx.x, before, hdr->scan);
         }
     }
-    if (!any) w.left = 0;
-    if (tid == 0) hdr->scan[34] = total, hdr->scan[35] = n_ctas;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = hdr->tmem_base;
 
-    auto give_up = [&](int code) {
-        if (!*cta_abort) {
-            raise_status(code);
-            *cta_abort = 1;
-        }
-    };
-    auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
-        if (wait_bar(bar, phase & 1u, cta_abort)) return true;
-        give_up(code);
-        return false;
+    auto wait = [&](uint64_t* bar, uint32_t phase, int code) { return wait_bar(bar, phase & 1u, code, cta_abort); };
+    // The next segment (number n of this CTA) as the planning warp has laid it down, and the return of its place; whole warps
+    auto have_seg = [&](int n) { return wait(&hdr->seg_full[n % AT_SEGS], n / AT_SEGS, DEV_TIMEOUT_FULL) && hdr->seg[n % AT_SEGS].valid; };
+    auto done_seg = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&hdr->seg_empty[n % AT_SEGS]));
     };
 
+    if (warp == AT_WARP_PLAN) {
+        // ------------------------------------------------------------ plan: the only code that knows how items follow one another
+        AtWalker w{p, 2 * tpt};
+        bool any = true;
+        if (p.stream_k) {
+            if (p.n_seqs <= AT_FEW_SEQS) {
+                warp_find_item<AtTiles>(p, 1l << 62, total);
+                n_ctas = ar_ctas(total, gridDim.x), share = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
+                first_seq = warp_find_item<AtTiles>(p, share, before);
+            }
+            if (lane == 0) {
+                (reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x)->n_rows = 0;
+                hdr->scan[34] = total, hdr->scan[35] = n_ctas;
+            }
+            any = (int)blockIdx.x < n_ctas && first_seq >= 0;
+            if (any) {
+                w.left = (int)(ar_share(total, blockIdx.x + 1, n_ctas) - share), w.s = first_seq;
+                w.load_seq();
+                const int ahead = (int)(share - before);  // (a sequence's tiles fit 31 bits: the entry point checks)
+                w.item = ahead / w.nt, w.within = ahead - w.item * w.nt;
+            }
+        } else {
+            w.s = first_seq, w.item = w.nb = w.within = 0, w.left = 1, w.ahead = blockIdx.x, w.turn = 0;
+            if (p.n_seqs > AT_FEW_SEQS) {
+                any = first_seq >= 0;
+                if (any) {
+                    w.load_seq();
+                    w.item = (int)(blockIdx.x - before), w.ahead = 0;
+                }
+            }
+        }
+        // It also clears the rows that were not loaded out of the value tiles (the tensor cores would add 0 * whatever was there):
+        // those of a segment after the next one is laid down.  The issuers ask for each such tile when it has landed and wait for
+        // it before they ask for the next: this warp does not follow the ring's own barriers, most of whose phases it would skip.
+        if (!any) {  // nothing to do for this CTA
+            if (lane == 0) {
+                hdr->seg[0].valid = 0;
+                mbar_arrive(smem_u32(&hdr->seg_full[0]));
+            }
+            __syncwarp();
+        }
+        int it = 0;
+        uint32_t n_v = 0;
+        AtSeg last = {};
+        bool ok = true;
+        for (int n = 0; ok && any; ++n) {
+            AtSeg g = {};
+            any = any && w.next(g);
+            if (n >= AT_SEGS && !wait(&hdr->seg_empty[n % AT_SEGS], n / AT_SEGS - 1, DEV_TIMEOUT_EMPTY)) break;
+            if (lane == 0) {
+                hdr->seg[n % AT_SEGS] = g;
+                mbar_arrive(smem_u32(&hdr->seg_full[n % AT_SEGS]));
+            }
+            __syncwarp();
+            for (int t = last.t0; t < last.t1; ++t, it += 2) {
+                if (!last.dirty(t)) continue;
+                const int sl = (it + 1) % Sh::SLOTS;
+                if (!wait(&hdr->v_ask, n_v++, DEV_TIMEOUT_FULL)) {
+                    ok = false;
+                    break;
+                }
+                uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)(2 + sl) * Sh::TILE_BYTES);
+                const int c0 = min(max(((last.a >> p.box_shift) << p.box_shift) - t * AT_TILE, 0), AT_TILE), c1 = max(min(last.kv - t * AT_TILE, AT_TILE), c0);
+#pragma unroll 1
+                for (int ch = 0; ch < Sh::NCH; ++ch) {
+                    for (int i = lane; i < c0 * 8; i += 32) vp[ch * AT_TILE * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
+                    for (int i = c1 * 8 + lane; i < AT_TILE * 8; i += 32) vp[ch * AT_TILE * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read by the tensor cores, refilled by a copy
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ok));
+            }
+            last = g;
+        }
+    } else
 
     if (warp == AT_WARP_COPY) {
         // ------------------------------------------------------------ copies
         int it = 0, q_no = 0;  // tiles (of keys and of values) and query blocks so far
         bool ok = true;
-        while (ok && w.next()) {
-            if (w.t0 >= w.t1) continue;
+        for (int n = 0; ok && have_seg(n); done_seg(n), ++n) {
+            const AtSeg& w = hdr->seg[n % AT_SEGS];
+            const int t0 = w.t0, t1 = w.t1, kvh = w.kvh, q0 = w.q0, kv_len = w.kv;
+            if (t0 >= t1) continue;
             const int nq = w.tok1 - w.tok0 > tpt ? 2 : 1;
             int first, cnt, pages, slots;
-            tile_boxes<AT_TILE>(p, w.t0, w.kr.a, w.si.kv, first, cnt);
-            pages = page_of_boxes<AT_TILE>(p, w.s, w.si.q0, w.t0, first, cnt, slots);
+            tile_boxes<AT_TILE>(p, t0, w.a, kv_len, first, cnt);
+            pages = page_of_boxes<AT_TILE>(p, w.s, q0, t0, first, cnt, slots);
             if (q_no > 0 && !wait(&hdr->q_empty, q_no - 1, DEV_TIMEOUT_EMPTY)) break;
             if (lane == 0) mbar_arrive_expect_tx(smem_u32(&hdr->q_full), (uint32_t)(nq * Sh::NCH * tile_rows * 128));
             __syncwarp();
             if (lane < nq * Sh::NCH) {
                 const int i = lane / Sh::NCH, c = lane % Sh::NCH;
-                tma_load_3d(q_s + (uint32_t)(i * Sh::TILE_BYTES + c * AT_TILE * 128), &qmap, c * 64, w.kvh * p.group, w.si.q0 + w.tok0 + i * tpt,
+                tma_load_3d(q_s + (uint32_t)(i * Sh::TILE_BYTES + c * AT_TILE * 128), &qmap, c * 64, kvh * p.group, q0 + w.tok0 + i * tpt,
                             smem_u32(&hdr->q_full));
             }
             ++q_no;
-            for (int t = w.t0; t < w.t1 && ok; ++t) {
+            for (int t = t0; t < t1 && ok; ++t) {
                 int nfirst = 0, ncnt = 0, npages = 0, nslots = 0;
-                if (t + 1 < w.t1) {  // the next tile's pages are looked up before its turn comes
-                    tile_boxes<AT_TILE>(p, t + 1, w.kr.a, w.si.kv, nfirst, ncnt);
-                    npages = page_of_boxes<AT_TILE>(p, w.s, w.si.q0, t + 1, nfirst, ncnt, nslots);
+                if (t + 1 < t1) {  // the next tile's pages are looked up before its turn comes
+                    tile_boxes<AT_TILE>(p, t + 1, w.a, kv_len, nfirst, ncnt);
+                    npages = page_of_boxes<AT_TILE>(p, w.s, q0, t + 1, nfirst, ncnt, nslots);
                 }
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv, ++it) {
@@ -419,7 +500,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                     const uint32_t bar = smem_u32(&hdr->full[sl]);
                     if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(cnt * Sh::NCH * 128) << p.box_shift);
                     __syncwarp();
-                    load_tile<AT_TILE, Sh::NCH>(p, kv ? &vmap : &kmap, ring + (uint32_t)sl * Sh::TILE_BYTES, bar, t, first, cnt, pages, slots, w.kvh);
+                    load_tile<AT_TILE, Sh::NCH>(p, kv ? &vmap : &kmap, ring + (uint32_t)sl * Sh::TILE_BYTES, bar, t, first, cnt, pages, slots, kvh);
                 }
                 first = nfirst, cnt = ncnt, pages = npages, slots = nslots;
             }
@@ -446,7 +527,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         const uint32_t d_s = tmem + AT_COL_S + 128u * i, d_o = tmem + AT_COL_O + 128u * i;
         const uint64_t qd = umma_desc_sw128(q_s + (uint32_t)i * Sh::TILE_BYTES);
         int it = 0, q_no = 0;
-        uint32_t n_p = 0, n_v = 0;  // P tiles awaited, value tiles handed to the clearing warp so far
+        uint32_t n_p = 0, n_v = 0;  // P tiles awaited, value tiles handed to the planning warp so far
         bool ok = true, active = false;
         auto mma_s = [&](int slot) {
             const uint64_t kd = umma_desc_sw128(ring + (uint32_t)slot * Sh::TILE_BYTES);
@@ -469,16 +550,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 else mbar_arrive(smem_u32(bar));
             }
         };
-        // a value tile with rows that were not loaded goes through the clearing warp while its scores are in softmax
-        auto ask_v = [&](int t, int v_it) {
-            if (!w.dirty(t)) return true;
+        // a value tile with rows that were not loaded goes through the planning warp while its scores are in softmax
+        auto ask_v = [&](bool dirty, int v_it) {
+            if (!dirty) return true;
             if (!wait(&hdr->full[v_it % Sh::SLOTS], v_it / Sh::SLOTS, DEV_TIMEOUT_FULL)) return false;
             if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ask));
             ++n_v;
             return true;
         };
-        while (ok && w.next()) {
-            if (w.t0 >= w.t1) continue;
+        for (int n = 0; ok && have_seg(n); done_seg(n), ++n) {
+            const AtSeg& w = hdr->seg[n % AT_SEGS];
+            const int t0 = w.t0, t1 = w.t1, d0 = w.d0, d1 = w.d1;
+            if (t0 >= t1) continue;
             active = i == 0 || w.tok1 - w.tok0 > tpt;
             int sl = it % Sh::SLOTS;
             if (!wait(&hdr->q_full, q_no, DEV_TIMEOUT_FULL) || !wait(&hdr->full[sl], it / Sh::SLOTS, DEV_TIMEOUT_FULL)) break;
@@ -486,20 +569,20 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
             tc_fence_after();
             if (active && lane == 0) mma_s(sl);
             release(&hdr->empty[sl]);
-            if (w.t0 + 1 == w.t1) release(&hdr->q_empty);
+            if (t0 + 1 == t1) release(&hdr->q_empty);
             ++it;
-            ok = ask_v(w.t0, it);
-            for (int t = w.t0; t < w.t1 && ok; ++t) {
+            ok = ask_v(t0 < d0 || t0 >= d1, it);
+            for (int t = t0; t < t1 && ok; ++t) {
                 const int vs = it % Sh::SLOTS, ks = (it + 1) % Sh::SLOTS;
-                const bool more = t + 1 < w.t1;
+                const bool more = t + 1 < t1;
                 ok = wait(&hdr->full[vs], it / Sh::SLOTS, DEV_TIMEOUT_FULL);
-                if (ok && w.dirty(t)) ok = wait(&hdr->v_ok, n_v - 1, DEV_TIMEOUT_FULL);
+                if (ok && (t < d0 || t >= d1)) ok = wait(&hdr->v_ok, n_v - 1, DEV_TIMEOUT_FULL);
                 if (ok && more) ok = wait(&hdr->full[ks], (it + 1) / Sh::SLOTS, DEV_TIMEOUT_FULL);
                 if (ok && active) {
                     ok = wait(&hdr->p_part[i], n_p, DEV_TIMEOUT_MMA);
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) mma_o(vs, 4, 8, t > w.t0);
+                    if (lane == 0) mma_o(vs, 4, 8, t > t0);
                     ok = wait(&hdr->p_full[i], n_p, DEV_TIMEOUT_MMA);
                     if (!ok) break;
                     ++n_p;
@@ -514,10 +597,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 release(&hdr->empty[vs]);
                 if (more) {
                     release(&hdr->empty[ks]);
-                    if (t + 2 == w.t1) release(&hdr->q_empty);
+                    if (t + 2 == t1) release(&hdr->q_empty);
                 }
                 it += more ? 2 : 1;
-                if (more) ok = ask_v(t + 1, it);
+                if (more) ok = ask_v(t + 1 < d0 || t + 1 >= d1, it);
             }
         }
         __syncwarp();
@@ -533,33 +616,6 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
             }
             __syncwarp();
         }
-    } else if (warp == AT_WARP_CLEAR) {
-        // ------------------------------------------------------------ value tiles with rows that were not loaded
-        // Those become zeros (the tensor cores would add 0 * whatever was there).  The issuers ask for each such tile when it has
-        // landed and wait for it before they ask for the next: this warp does not follow the ring's own barriers, most of whose
-        // phases it would skip.
-        int it = 0;
-        uint32_t n_v = 0;
-        bool ok = true;
-        while (ok && w.next()) {
-            for (int t = w.t0; t < w.t1; ++t, it += 2) {
-                if (!w.dirty(t)) continue;
-                const int sl = (it + 1) % Sh::SLOTS;
-                if (!wait(&hdr->v_ask, n_v++, DEV_TIMEOUT_FULL)) {
-                    ok = false;
-                    break;
-                }
-                uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)(2 + sl) * Sh::TILE_BYTES);
-                const int c0 = min(max(((w.kr.a >> p.box_shift) << p.box_shift) - t * AT_TILE, 0), AT_TILE), c1 = max(min(w.si.kv - t * AT_TILE, AT_TILE), c0);
-                for (int ch = 0; ch < Sh::NCH; ++ch) {
-                    for (int i = lane; i < c0 * 8; i += 32) vp[ch * AT_TILE * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
-                    for (int i = c1 * 8 + lane; i < AT_TILE * 8; i += 32) vp[ch * AT_TILE * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read by the tensor cores, refilled by a copy
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ok));
-            }
-        }
     } else {
         // ------------------------------------------------------------ softmax and epilogue: 16 rows per warp
         const int wg = warp >> 3, row0 = (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + (lane >> 2);  // this lane's rows: row0, row0 + 8
@@ -568,20 +624,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         uint32_t n_s = 0, n_o = 0, n_turn = 0;
         const float c = p.scale_log2;
         bool ok = true;
-        while (ok && w.next()) {
+        for (int n = 0; ok && have_seg(n); done_seg(n), ++n) {
+            const AtSeg& w = hdr->seg[n % AT_SEGS];
+            const int t0 = w.t0, t1 = w.t1, u0 = w.u0, u1 = w.u1, pos0 = w.kv - w.q_len;
             const int n_tok = w.tok1 - w.tok0;
             const bool both = n_tok > tpt;
             if (wg == 1 && !both) continue;  // no rows in this row tile
             int lo[2], hi[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int tok = w.tok0 + wg * tpt + ((row0 + 8 * e) * p.group_inv >> 16), pos = w.si.kv - w.si.q_len + tok;
+                const int tok = w.tok0 + wg * tpt + ((row0 + 8 * e) * p.group_inv >> 16), pos = pos0 + tok;
                 hi[e] = row0 + 8 * e < tile_rows && tok < w.tok1 ? max(pos + 1, 0) : 0;
                 lo[e] = p.window ? max(0, pos - p.window + 1) : 0;
             }
             float m[2] = {-INFINITY, -INFINITY};
             uint64_t l2[2] = {0ull, 0ull};  // sums of this lane's even and odd columns
-            for (int t = w.t0; t < w.t1; ++t) {
+            for (int t = t0; t < t1; ++t) {
                 if (!wait(&hdr->s_full[wg], n_s, DEV_TIMEOUT_MMA)) {
                     ok = false;
                     break;
@@ -590,7 +648,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 tc_fence_after();
                 // The rows' maxima from both halves of the keys; the second half stays in registers, the first is read again for
                 // its exponentials
-                const bool right = t >= w.u1, left = t < w.u0;
+                const bool right = t >= u1, left = t < u0;
                 uint32_t sr[32];
                 float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
@@ -607,7 +665,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                     mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 2));
                     grew |= (mt[e] - m[e]) * c > 8.f || (m[e] == -INFINITY && mt[e] > -INFINITY);
                 }
-                if (t == w.t0) {
+                if (t == t0) {
                     m[0] = mt[0], m[1] = mt[1];
                 } else if (__any_sync(0xffffffffu, grew)) {
                     float f[2];
@@ -653,7 +711,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 if (both && lane == 0) mbar_arrive(smem_u32(&hdr->turn[wg ^ 1][warp & 3]));
             }
             if (!ok) break;
-            if (w.t0 < w.t1) {
+            if (t0 < t1) {
                 if (!wait(&hdr->o_full[wg], n_o, DEV_TIMEOUT_MMA)) break;
                 ++n_o;
                 tc_fence_after();
@@ -663,73 +721,72 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
             float* ml = whole ? nullptr : ArScratch<HD, AT_MAX_ROWS>::ml(p.scratch, gridDim.x, slot);
             float* so = whole ? nullptr : ArScratch<HD, AT_MAX_ROWS>::o(p.scratch, gridDim.x, slot);
             {
-                // f32 (and what is joined later): 8 bytes per lane, 32-byte pieces; 16-bit outputs of 32 columns are turned within
-                // the four lanes of a row, 16 bytes per lane, 64-byte pieces
-                const bool f32 = !whole || p.out_dtype == QMM_DT_F32;
-                const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % 8 == 0;
+                // each lane its own columns, 8 or 4 bytes a time (turning them within the four lanes of a row for wider stores took
+                // three times the instructions, which are what bounds this part)
                 char* dst[2];
-                float inv[2];
-                bool live[2], sees[2];
+                uint64_t inv[2], odd[2] = {0ull, 0ull};
+                bool live[2];
+                const bool f32 = !whole || p.out_dtype == QMM_DT_F32, f16 = p.out_dtype == QMM_DT_F16;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int row = row0 + 8 * e, tk = row * p.group_inv >> 16, g = row - tk * p.group, tok = w.tok0 + wg * tpt + tk;
                     float l = lo2(l2[e]) + hi2(l2[e]);
                     l += __shfl_xor_sync(0xffffffffu, l, 1);
                     l += __shfl_xor_sync(0xffffffffu, l, 2);
-                    live[e] = row < tile_rows && tok < w.tok1, sees[e] = w.si.kv - w.si.q_len + tok >= 0;
-                    inv[e] = whole ? 1.f / l : 1.f;
+                    live[e] = row < tile_rows && tok < w.tok1;
+                    const float i = !whole ? 1.f : pos0 + tok >= 0 ? 1.f / l : 0.f;  // (a row that sees no key has zeros)
+                    inv[e] = f32x2(i, i);
                     const int r = (tok - w.tok0) * p.group + g;  // row of the item
-                    const size_t oe = (size_t)(w.si.q0 + tok) * p.out_stride + (size_t)(w.kvh * p.group + g) * HD;
-                    dst[e] = whole ? static_cast<char*>(p.out) + oe * (f32 ? 4 : 2) : reinterpret_cast<char*>(so + (size_t)r * HD);
+                    const size_t oe = (size_t)(w.q0 + tok) * p.out_stride + (size_t)(w.kvh * p.group + g) * HD;
+                    dst[e] = (whole ? static_cast<char*>(p.out) + oe * (f32 ? 4 : 2) : reinterpret_cast<char*>(so + (size_t)r * HD)) + (lane & 3) * (f32 ? 8 : 4);
                     if (!whole && live[e] && (lane & 3) == 0) ml[2 * r] = m[e], ml[2 * r + 1] = l;
                 }
-                float odd[2] = {0.f, 0.f};
 #pragma unroll 2
                 for (int q = 0; q < HD / 32; ++q) {
                     uint32_t o[16];
-                    if (w.t0 < w.t1) {
+                    if (t0 < t1) {
                         tmem_ld_4(to + 32 * q, o);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 16; ++j) o[j] = 0u;
                     }
+                    uint64_t v[8];  // block i of 8 columns, row e: v[2 i + e]
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) odd[(j >> 1) & 1] += __uint_as_float(o[j]) * 0.f;
+                    for (int j = 0; j < 8; ++j) {
+                        const uint64_t x = f32x2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
+                        odd[j & 1] = fma2(x, 0ull, odd[j & 1]);  // 0 * x is 0, or NaN where x is not finite
+                        v[j] = mul2(x, inv[j & 1]);
+                    }
+                    if (f32) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float v[8];
+                        for (int j = 0; j < 8; ++j)
+                            if (live[j & 1]) *reinterpret_cast<float2*>(dst[j & 1] + (32 * q + 8 * (j >> 1)) * 4) = make_float2(lo2(v[j]), hi2(v[j]));
+                    } else {
+                        uint32_t h[8];
+                        if (f16) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = whole && !sees[e] ? 0.f : __uint_as_float(o[4 * (j >> 1) + 2 * e + (j & 1)]) * inv[e];
-                        if (f32) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (live[e]) *reinterpret_cast<float2*>(dst[e] + (32 * q + 8 * i + 2 * (lane & 3)) * 4) = make_float2(v[2 * i], v[2 * i + 1]);
+                            for (int j = 0; j < 8; ++j) h[j] = pack2<__half>(lo2(v[j]), hi2(v[j]));
                         } else {
-                            uint32_t h[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                h[i] = p.out_dtype == QMM_DT_F16 ? pack2<__half>(v[2 * i], v[2 * i + 1]) : pack2<__nv_bfloat16>(v[2 * i], v[2 * i + 1]);
-                            if (vec) {
-                                turn4(h);
-                                if (live[e]) *reinterpret_cast<uint4*>(dst[e] + (32 * q + 8 * (lane & 3)) * 2) = make_uint4(h[0], h[1], h[2], h[3]);
-                            } else if (live[e]) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(dst[e] + (32 * q + 8 * i + 2 * (lane & 3)) * 2) = h[i];
-                            }
+                            for (int j = 0; j < 8; ++j) h[j] = pack2<__nv_bfloat16>(lo2(v[j]), hi2(v[j]));
                         }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (live[j & 1]) *reinterpret_cast<uint32_t*>(dst[j & 1] + (32 * q + 8 * (j >> 1)) * 2) = h[j];
                     }
                 }
                 // outputs that are not finite: from a value that the row does not see, or by the formula; either way again, exactly
-                if (__any_sync(0xffffffffu, (live[0] && odd[0] != odd[0]) || (live[1] && odd[1] != odd[1])))
+                const float odd0 = lo2(odd[0]) + hi2(odd[0]), odd1 = lo2(odd[1]) + hi2(odd[1]);
+                if (__any_sync(0xffffffffu, (live[0] && odd0 != odd0) || (live[1] && odd1 != odd1)))
                     at_exact_rows<T, HD>(p, w, wg * tpt, row0 - (lane >> 2), tile_rows, whole, so, ml);
             }
             if (w.begins && !w.ends && tid == 0) {  // this item goes on in the next CTAs: how many of them
                 ArJoin j;
-                j.s = w.s, j.q0 = w.si.q0, j.tok_row0 = w.tok0 * p.group, j.n_rows = n_tok * p.group, j.kvh = w.kvh;
-                j.any_key = w.si.kv - w.si.q_len;
+                j.s = w.s, j.q0 = w.q0, j.tok_row0 = w.tok0 * p.group, j.n_rows = n_tok * p.group, j.kvh = w.kvh;
+                j.any_key = pos0;
                 const long total = hdr->scan[34];
                 const int n_ctas = (int)hdr->scan[35];
-                const long item_end = ar_share(total, blockIdx.x + 1, n_ctas) + (w.nt - (w.st1 - w.tl));
+                const long item_end = ar_share(total, blockIdx.x + 1, n_ctas) + w.more;  // (a segment that does not end its item ends the share)
                 int e = blockIdx.x + 1;
                 while (ar_share(total, e + 1, n_ctas) < item_end) ++e;
                 j.n_parts = e - (int)blockIdx.x + 1, j.pad = 0;
