@@ -30,8 +30,23 @@ template <int HD, int WM> struct ArShape {
     static constexpr bool Q_REGS = HD <= 128;  // the queries stay in registers (wider heads read them from shared memory)
 };
 
+constexpr int AR_SEGS = 4;  // segments planned ahead
+// A segment: some of the key tiles of an item, as the copying warp hands it to the math warps
+struct ArSeg {
+    int valid;            // 0: no more
+    int s, q0, q_len, kv, kvh;
+    int r0, n_rows;       // rows r0 .. + n_rows of the sequence's (token, head of the group) list
+    int t0, t1;           // tiles [t0, t1) that hold keys of the rows
+    int st0, st1;         // tiles of the segment before that cut
+    int a2, b2;           // keys [a2, b2) are seen by every row
+    int c0;               // first key that is loaded
+    int begins, ends;     // the item's first / last segment
+    int more;             // tiles of the item after the segment
+};
+
 struct __align__(16) ArHeader {
-    uint64_t full[8], empty[8];
+    uint64_t full[8], empty[8], seg_full[AR_SEGS], seg_empty[AR_SEGS], q_full, q_empty;
+    ArSeg seg[AR_SEGS];
     long long scan[36];
     float ml[4][16][2];
     AttnParams p;  // a copy: functions that are not inlined would fetch the kernel's parameters from far away, one by one
@@ -76,18 +91,15 @@ __device__ __forceinline__ bool bar_any(bool x) {
 }
 __device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// Walks the segments (item, tiles [t0, t1) of it) of this CTA; every thread of the CTA runs it and gets the same segments.
-// An item is (sequence, kv head, block of R rows); all items of a sequence count the tiles of the whole sequence, at least one.
+// Walks the segments (item, tiles of it) of this CTA (the copying warp).  An item is (sequence, kv head, block of R rows); all items
+// of a sequence count the tiles of the whole sequence, at least one.
 template <int R>
 struct ArWalker {
     const AttnParams& p;
-    long g, g1;        // this CTA's share of all tiles: [g, g1)
+    long left;         // tiles of this CTA's share still to come
     int s, item, within;
     SeqInfo si;
     int tl, nt, nrb;   // of sequence s: first tile, tiles per item, row blocks
-    // of the current segment
-    int t0, t1, kvh, rb;
-    bool begins, ends;
 
     __device__ __forceinline__ void load_seq() {
         si = seq_info(p, s);
@@ -96,19 +108,24 @@ struct ArWalker {
         nt = max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - tl);
         nrb = (si.q_len * p.group + R - 1) / R;
     }
-    __device__ __noinline__ bool next() {
-        if (g >= g1) return false;
+    __device__ __forceinline__ bool next(ArSeg& g) {
+        if (left <= 0) return false;
         while (item >= nrb * p.nkv) {  // (sequences without rows have no items)
             if (++s >= p.n_seqs) return false;
             item = within = 0;
             load_seq();
         }
-        const int n = (int)min(g1 - g, (long)(nt - within));
-        kvh = item / nrb, rb = item - kvh * nrb;
-        t0 = tl + within, t1 = t0 + n;
-        begins = within == 0, ends = within + n == nt;
-        g += n, within += n;
+        const int n = (int)min(left, (long)(nt - within)), rb = item % nrb;
+        g.valid = 1, g.s = s, g.q0 = si.q0, g.q_len = si.q_len, g.kv = si.kv, g.kvh = item / nrb;
+        g.st0 = tl + within, g.st1 = g.st0 + n;
+        g.begins = within == 0, g.ends = within + n == nt;
+        left -= n, within += n;
+        g.more = nt - within;
         if (within == nt) within = 0, ++item;
+        g.r0 = rb * R, g.n_rows = min(R, si.q_len * p.group - g.r0);
+        const KeyRange kr = key_range(p, si, g.r0 / p.group, (g.r0 + g.n_rows - 1) / p.group + 1);
+        g.t0 = max(g.st0, kr.a / AR_TILE), g.t1 = min(g.st1, (kr.b + AR_TILE - 1) / AR_TILE);
+        g.a2 = kr.a2, g.b2 = kr.b2, g.c0 = (kr.a >> p.box_shift) << p.box_shift;
         return true;
     }
 };
@@ -152,6 +169,8 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
 
     if (tid == 0) {
         for (int i = 0; i < Sh::STAGES; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), 4);
+        for (int i = 0; i < AR_SEGS; ++i) mbar_init(smem_u32(&hdr->seg_full[i]), 1), mbar_init(smem_u32(&hdr->seg_empty[i]), 4);
+        mbar_init(smem_u32(&hdr->q_full), 1), mbar_init(smem_u32(&hdr->q_empty), 4);
         hdr->abort_flag = 0;
         mbar_fence_init();
     }
@@ -160,75 +179,83 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
     pdl_wait_prior_grids();
     pdl_release_dependents();
 
-    ArWalker<R> w{p};
-    int n_ctas = 1;
-    long total = 0;  // tiles of the whole batch (shared evenly)
+    int n_ctas = 1, first_seq;
+    long total = 0, before = 0, share = 0;  // tiles of the whole batch, before the sequence and before this CTA's share
     if (p.stream_k) {
-        // all tiles, then the sequence this CTA's share starts in
-        long before = 0;
         find_item<ArTiles<R>>(p, 1l << 62, total, hdr->scan);
         n_ctas = ar_ctas(total, gridDim.x);
-        ArJoin* join = reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x;
-        if (tid == 0) join->n_rows = 0;
+        if (tid == 0) (reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x)->n_rows = 0;
         if ((int)blockIdx.x >= n_ctas) return;
-        w.g = ar_share(total, blockIdx.x, n_ctas), w.g1 = ar_share(total, blockIdx.x + 1, n_ctas);
-        w.s = find_item<ArTiles<R>>(p, w.g, before, hdr->scan);
-        if (w.s < 0) return;  // (no rows at all)
-        w.load_seq();
-        w.item = (int)((w.g - before) / w.nt), w.within = (int)((w.g - before) % w.nt);
+        share = ar_share(total, blockIdx.x, n_ctas);
+        first_seq = find_item<ArTiles<R>>(p, share, before, hdr->scan);
     } else {
-        // one item per CTA: block row blockIdx.y of all row blocks (a sequence's last, longest, first), kv head blockIdx.x
-        long before = 0;
-        w.s = find_item<ArBlocks<R>>(p, blockIdx.y, before, hdr->scan);
-        if (w.s < 0) return;
-        w.load_seq();
-        w.g = 0, w.g1 = w.nt, w.within = 0;
-        w.item = blockIdx.x * w.nrb + (w.nrb - 1 - (int)(blockIdx.y - before));
+        first_seq = find_item<ArBlocks<R>>(p, blockIdx.y, before, hdr->scan);
     }
+    if (first_seq < 0) return;  // (no rows at all, or no such block)
     __syncthreads();
     int it = 0;  // tiles so far, over all segments: stage it % STAGES
 
-    // the tokens of a row block, and the tiles of a segment that hold keys of its rows
-    auto block_range = [&](int& tok0, int& n_rows, KeyRange& kr, int& t0, int& t1) {
-        const int r0 = w.rb * R;
-        n_rows = min(R, w.si.q_len * p.group - r0);
-        tok0 = r0 / p.group;
-        kr = key_range(p, w.si, tok0, (r0 + n_rows - 1) / p.group + 1);
-        t0 = max(w.t0, kr.a / AR_TILE), t1 = min(w.t1, (kr.b + AR_TILE - 1) / AR_TILE);
-    };
-
     if (warp == 4) {
-        // ------------------------------------------------------------ copies
-        while (!*cta_abort && w.next()) {
-            int tok0, n_rows, t0, t1;
-            KeyRange kr;
-            block_range(tok0, n_rows, kr, t0, t1);
-            int first, count, slots = 0, pages = 0;
-            if (t0 < t1) {
-                tile_boxes<AR_TILE>(p, t0, kr.a, w.si.kv, first, count);
-                pages = page_of_boxes<AR_TILE>(p, w.s, w.si.q0, t0, first, count, slots);
+        // ------------------------------------------------------------ plan and copies
+        ArWalker<R> w{p};
+        w.s = first_seq;
+        w.load_seq();
+        if (p.stream_k) {
+            w.left = ar_share(total, blockIdx.x + 1, n_ctas) - share;
+            const int ahead = (int)(share - before);
+            w.item = ahead / w.nt, w.within = ahead - w.item * w.nt;
+        } else {  // one item per CTA: row block blockIdx.y of all (a sequence's last, longest, first), kv head blockIdx.x
+            w.left = w.nt, w.within = 0;
+            w.item = blockIdx.x * w.nrb + (w.nrb - 1 - (int)(blockIdx.y - before));
+        }
+        int q_no = 0;
+        for (int n = 0; !*cta_abort; ++n) {
+            ArSeg g = {};
+            const bool any = w.next(g);
+            if (n >= AR_SEGS && !wait_bar(&hdr->seg_empty[n % AR_SEGS], (n / AR_SEGS - 1) & 1, DEV_TIMEOUT_EMPTY, cta_abort)) break;
+            if (lane == 0) {
+                hdr->seg[n % AR_SEGS] = g;
+                mbar_arrive(smem_u32(&hdr->seg_full[n % AR_SEGS]));
             }
-            for (int t = t0; t < t1; ++t, ++it) {
+            if (!any) break;
+            // queries: a row of HD elements at a time; the math warps have taken the ones before to their registers
+            if (n > 0 && !wait_bar(&hdr->q_empty, (n - 1) & 1, DEV_TIMEOUT_EMPTY, cta_abort)) break;
+            if (lane == 0) mbar_arrive_expect_tx(smem_u32(&hdr->q_full), (uint32_t)(g.n_rows * HD * 2));
+            __syncwarp();
+            q_no = n + 1;
+            for (int r = lane; r < g.n_rows; r += 32) {
+                const int tok = (g.r0 + r) / p.group, h = g.kvh * p.group + (g.r0 + r) - tok * p.group;
+                bulk_g2s(smem_u32(qs + r * QPITCH), static_cast<const T*>(p.q) + (size_t)(g.q0 + tok) * p.q_stride + (size_t)h * HD, HD * 2, smem_u32(&hdr->q_full));
+            }
+            int first, count, slots = 0, pages = 0;
+            if (g.t0 < g.t1) {
+                tile_boxes<AR_TILE>(p, g.t0, g.c0, g.kv, first, count);
+                pages = page_of_boxes<AR_TILE>(p, g.s, g.q0, g.t0, first, count, slots);
+            }
+            for (int t = g.t0; t < g.t1; ++t, ++it) {
                 const int st = it % Sh::STAGES;
                 int nfirst = 0, ncount = 0, npages = 0, nslots = 0;
-                if (t + 1 < t1) {  // the next tile's pages are looked up before this tile's turn comes
-                    tile_boxes<AR_TILE>(p, t + 1, kr.a, w.si.kv, nfirst, ncount);
-                    npages = page_of_boxes<AR_TILE>(p, w.s, w.si.q0, t + 1, nfirst, ncount, nslots);
+                if (t + 1 < g.t1) {  // the next tile's pages are looked up before this tile's turn comes
+                    tile_boxes<AR_TILE>(p, t + 1, g.c0, g.kv, nfirst, ncount);
+                    npages = page_of_boxes<AR_TILE>(p, g.s, g.q0, t + 1, nfirst, ncount, nslots);
                 }
                 if (it >= Sh::STAGES && !wait_bar(&hdr->empty[st], ((it / Sh::STAGES) - 1) & 1, DEV_TIMEOUT_EMPTY, cta_abort)) break;
                 const uint32_t bar = smem_u32(&hdr->full[st]), dst = ring + (uint32_t)st * 2 * Sh::TILE_BYTES;
                 if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(count * 2 * Sh::NCH * 128) << p.box_shift);
                 __syncwarp();
-                load_tile<AR_TILE, Sh::NCH>(p, &kmap, dst, bar, t, first, count, pages, slots, w.kvh);
-                load_tile<AR_TILE, Sh::NCH>(p, &vmap, dst + Sh::TILE_BYTES, bar, t, first, count, pages, slots, w.kvh);
+                load_tile<AR_TILE, Sh::NCH>(p, &kmap, dst, bar, t, first, count, pages, slots, g.kvh);
+                load_tile<AR_TILE, Sh::NCH>(p, &vmap, dst + Sh::TILE_BYTES, bar, t, first, count, pages, slots, g.kvh);
                 first = nfirst, count = ncount, pages = npages, slots = nslots;
             }
         }
-        // copies in flight land before the CTA ends (on every path: after a normal run the consumers have seen them all)
+        // copies in flight land before the CTA ends (after a normal run the math warps have seen them all)
         if (*cta_abort) {
-            for (int i = max(0, it - Sh::STAGES); i < it; ++i) {
+#pragma unroll 1
+            for (int i = max(0, it - Sh::STAGES); i <= it; ++i) {
+                if (i == it && q_no == 0) break;
+                const uint32_t bar = smem_u32(i < it ? &hdr->full[i % Sh::STAGES] : &hdr->q_full), ph = (i < it ? i / Sh::STAGES : q_no - 1) & 1;
                 const long long c0 = clock64();
-                while (!mbar_try_wait(smem_u32(&hdr->full[i % Sh::STAGES]), (i / Sh::STAGES) & 1))
+                while (!mbar_try_wait(bar, ph))
                     if (clock64() - c0 > WAIT_LIMIT_CYCLES) {
                         raise_status(DEV_TIMEOUT_DRAIN);
                         break;
@@ -241,29 +268,21 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
     // ---------------------------------------------------------------- math warps
     const int qr = lane >> 2, pq = lane & 3;
     const int row_w = WM == 1 ? 0 : 16 * warp, key_w = WM == 1 ? KW * warp : 0;  // this warp's rows and keys of a tile
-    while (w.next()) {
-        int tok0, n_rows, t0, t1;
-        KeyRange kr;
-        block_range(tok0, n_rows, kr, t0, t1);
-        const int r0 = w.rb * R;
-        // queries to shared memory (elements past HD and rows past the block: zeros), then to registers as A fragments
-        math_sync();  // the fragments and the buffer of the segment before have been read
-        for (int i = tid; i < R * Sh::NCH * 8; i += 128) {
-            const int r = i / (Sh::NCH * 8), c = (i - r * (Sh::NCH * 8)) * 8;
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (r < n_rows && c < HD) {
-                const int tok = (r0 + r) / p.group, h = w.kvh * p.group + (r0 + r) % p.group;
-                x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (size_t)(w.si.q0 + tok) * p.q_stride + (size_t)h * HD + c);
-            }
-            *reinterpret_cast<uint4*>(qs + r * QPITCH + c) = x;
-        }
-        math_sync();
+    for (int sn = 0;; ++sn) {
+        // (a wait that runs out does not end a math warp's run over the segments it knows of: the warps meet at barriers; without
+        // a next segment all four stop alike)
+        if (!wait_bar(&hdr->seg_full[sn % AR_SEGS], (sn / AR_SEGS) & 1, DEV_TIMEOUT_FULL, cta_abort)) hdr->seg[sn % AR_SEGS].valid = 0;
+        math_sync();  // (also: the buffer of the segment before has been read)
+        const ArSeg& w = hdr->seg[sn % AR_SEGS];
+        if (!w.valid) break;
+        const int n_rows = w.n_rows, t0 = w.t0, t1 = w.t1, r0 = w.r0, pos0 = w.kv - w.q_len, kv_len = w.kv;
+        wait_bar(&hdr->q_full, sn & 1, DEV_TIMEOUT_FULL, cta_abort);
         // this thread's two rows: the keys [lo, hi) they see
         int lo[2], hi[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int r = row_w + qr + 8 * e;
-            const int pos = w.si.kv - w.si.q_len + (r0 + r) / p.group;
+            const int pos = pos0 + (r0 + r) / p.group;
             hi[e] = r < n_rows ? max(pos + 1, 0) : 0;
             lo[e] = p.window ? max(0, pos - p.window + 1) : 0;
         }
@@ -272,6 +291,8 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
         if constexpr (Sh::Q_REGS) {
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk) ldsm_x4(qf[kk], qa + kk * 32);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&hdr->q_empty));
         }
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
         float o[HD / 8][4];
@@ -283,8 +304,8 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
             wait_bar(&hdr->full[st], (it / Sh::STAGES) & 1, DEV_TIMEOUT_FULL, cta_abort);  // (on to the end even if it runs out: the warps meet at barriers)
             const uint32_t ks = ring + (uint32_t)st * 2 * Sh::TILE_BYTES, vs = ks + Sh::TILE_BYTES;
             const int k0 = t * AR_TILE;
-            const bool masked = k0 < kr.a2 || k0 + AR_TILE > kr.b2;  // some row does not see some key of the tile
-            const int c0 = ((kr.a >> p.box_shift) << p.box_shift) - k0, c1 = w.si.kv - k0;  // keys of the tile outside [c0, c1): not loaded
+            const bool masked = k0 < w.a2 || k0 + AR_TILE > w.b2;  // some row does not see some key of the tile
+            const int c0 = w.c0 - k0, c1 = kv_len - k0;  // keys of the tile outside [c0, c1): not loaded
             if (c0 > 0 || c1 < AR_TILE) {
                 uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)st * 2 * Sh::TILE_BYTES + Sh::TILE_BYTES);
                 for (int i = tid; i < Sh::NCH * AR_TILE * 8; i += 128) {
@@ -375,6 +396,10 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
         }
 
+        if constexpr (!Sh::Q_REGS) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&hdr->q_empty));
+        }
         // where the segment's result goes: the output rows, or a slot of scratch (0: continues an item, 1: begins one)
         const bool whole = w.begins && w.ends;
         const int slot = 2 * (int)blockIdx.x + (w.begins ? 1 : 0);
@@ -382,22 +407,22 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
         float* so = whole ? nullptr : ArScratch<HD, R>::o(p.scratch, gridDim.x, slot);
         auto out_elem = [&](int r) {  // element index of row r's first output
             const int tok = (r0 + r) / p.group, h = w.kvh * p.group + (r0 + r) % p.group;
-            return (size_t)(w.si.q0 + tok) * p.out_stride + (size_t)h * HD;
+            return (size_t)(w.q0 + tok) * p.out_stride + (size_t)h * HD;
         };
         auto row_sees = [&](int r) {  // row r has keys at all (else its output is 0)
-            return w.si.kv - w.si.q_len + (r0 + r) / p.group >= 0;
+            return pos0 + (r0 + r) / p.group >= 0;
         };
         // outputs that are not finite: from a value that the row does not see, or by the formula; either way again, exactly
-        float odd = 0.f;
+        float odd[2] = {0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n) odd += (o[n][0] + o[n][1]) * 0.f + (o[n][2] + o[n][3]) * 0.f;
-        if (bar_any(odd != odd)) {
+        for (int i = 0; i < HD / 8; ++i) odd[0] += (o[i][0] + o[i][1]) * 0.f, odd[1] += (o[i][2] + o[i][3]) * 0.f;
+        if (bar_any((odd[0] != odd[0] && row_w + qr < n_rows) || (odd[1] != odd[1] && row_w + qr + 8 < n_rows))) {
 #pragma unroll 1
             for (int r = warp; r < n_rows; r += 4) {
-                const int tok = (r0 + r) / p.group, pos = w.si.kv - w.si.q_len + tok;
+                const int tok = (r0 + r) / p.group, pos = pos0 + tok;
                 float em, el, eo[HD / 32];
-                attn_row_exact<T, HD>(p, w.s, w.si.q0, tok, w.kvh * p.group + (r0 + r) % p.group, w.kvh,
-                                      max(w.t0 * AR_TILE, p.window ? max(0, pos - p.window + 1) : 0), min(w.t1 * AR_TILE, pos + 1), em, el, eo);
+                attn_row_exact<T, HD>(p, w.s, w.q0, tok, w.kvh * p.group + (r0 + r) % p.group, w.kvh,
+                                      max(w.st0 * AR_TILE, p.window ? max(0, pos - p.window + 1) : 0), min(w.st1 * AR_TILE, pos + 1), em, el, eo);
                 const float inv = 1.f / el;
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) {
@@ -470,14 +495,16 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
         if (w.begins && !w.ends && tid == 0) {
             // this item goes on in the next CTAs: how many of them
             ArJoin j;
-            j.s = w.s, j.q0 = w.si.q0, j.tok_row0 = r0, j.n_rows = n_rows, j.kvh = w.kvh;
-            j.any_key = w.si.kv - w.si.q_len;  // position of token 0
-            const long item_end = w.g1 + (w.nt - (w.t1 - w.tl));  // (a segment that does not end its item ends the share)
+            j.s = w.s, j.q0 = w.q0, j.tok_row0 = r0, j.n_rows = n_rows, j.kvh = w.kvh;
+            j.any_key = pos0;  // position of token 0
+            const long item_end = ar_share(total, blockIdx.x + 1, n_ctas) + w.more;  // (a segment that does not end its item ends the share)
             int c = blockIdx.x + 1;
             while (ar_share(total, c + 1, n_ctas) < item_end) ++c;
             j.n_parts = c - (int)blockIdx.x + 1, j.pad = 0;
             reinterpret_cast<ArJoin*>(p.scratch)[blockIdx.x] = j;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&hdr->seg_empty[sn % AR_SEGS]));
     }
 }
 
