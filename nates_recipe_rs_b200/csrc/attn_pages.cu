@@ -109,7 +109,9 @@ int launch_rope_kv_append_paged(const void* qkv, int qkv_dtype, long qkv_stride,
     p.table_stride = kv->table_stride, p.page_size = kv->page_size, p.n_pages = kv->n_pages;
     p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = seqs->max_kv;
     p.nqh = n_q_heads, p.nkv = nkv, p.hd = hd, p.half = rotary_dim / 2;
-    for (int j = 0; j < p.half; ++j) p.freq[j] = std::pow((double)theta, -2.0 * j / rotary_dim);
+    const double step = rotary_dim ? std::pow((double)theta, -2.0 / rotary_dim) : 1.0;
+    p.freq[0] = 1.0;  // (127 products in f64 are off by at most 127 * 2^-53 relative)
+    for (int j = 1; j < p.half; ++j) p.freq[j] = p.freq[j - 1] * step;
     // 16-byte accesses where every head, half head and row begins on one
     const bool wide = p.half % 8 == 0 && hd % 8 == 0 && !misaligned(qkv, 16) && !misaligned(q_out, 16) && qkv_stride * size_in % 16 == 0;
     // enough tokens per CTA that its threads have two units of work each, as long as every SM keeps several CTAs

@@ -31,6 +31,7 @@ template <int HD, int WM> struct ArShape {
 };
 
 constexpr int AR_SEGS = 4;  // segments planned ahead
+constexpr int AR_FEW_SEQS = 64;
 // A segment: some of the key tiles of an item, as the copying warp hands it to the math warps
 struct ArSeg {
     int valid;            // 0: no more
@@ -91,12 +92,17 @@ __device__ __forceinline__ bool bar_any(bool x) {
 }
 __device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
+__device__ __forceinline__ int ar_tile_count(const KeyRange& kr) { return max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - kr.a / AR_TILE); }
+constexpr int AR_ITEM_COST = 2;
+
 // Walks the segments (item, tiles of it) of this CTA (the copying warp).  An item is (sequence, kv head, block of R rows); all items
-// of a sequence count the tiles of the whole sequence, at least one.
+// of a sequence count the tiles of the whole sequence, at least one, and AR_ITEM_COST more for what an item costs beside its tiles
+// (its queries, the joining of its warps, its outputs): without that the CTAs that got the short sequences finished last.  A share
+// that begins or ends among those extra places begins or ends where the item does.
 template <int R>
 struct ArWalker {
     const AttnParams& p;
-    long left;         // tiles of this CTA's share still to come
+    long left;         // places of this CTA's share still to come
     int s, item, within;
     SeqInfo si;
     int tl, nt, nrb;   // of sequence s: first tile, tiles per item, row blocks
@@ -105,7 +111,7 @@ struct ArWalker {
         si = seq_info(p, s);
         const KeyRange kr = key_range(p, si, 0, si.q_len);
         tl = kr.a / AR_TILE;
-        nt = max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - tl);
+        nt = ar_tile_count(kr);
         nrb = (si.q_len * p.group + R - 1) / R;
     }
     __device__ __forceinline__ bool next(ArSeg& g) {
@@ -115,13 +121,15 @@ struct ArWalker {
             item = within = 0;
             load_seq();
         }
-        const int n = (int)min(left, (long)(nt - within)), rb = item % nrb;
+        if (within == 0 && left <= AR_ITEM_COST) return false;  // (its first places: the item is the next CTA's)
+        if (within > 0 && within <= AR_ITEM_COST) left += within, within = 0;
+        const int n = (int)min(left, (long)(nt + AR_ITEM_COST - within)), rb = item % nrb, w1 = within + n;
         g.valid = 1, g.s = s, g.q0 = si.q0, g.q_len = si.q_len, g.kv = si.kv, g.kvh = item / nrb;
-        g.st0 = tl + within, g.st1 = g.st0 + n;
-        g.begins = within == 0, g.ends = within + n == nt;
-        left -= n, within += n;
-        g.more = nt - within;
-        if (within == nt) within = 0, ++item;
+        g.begins = within == 0, g.ends = w1 == nt + AR_ITEM_COST;
+        g.st0 = tl + max(0, within - AR_ITEM_COST), g.st1 = tl + w1 - AR_ITEM_COST;
+        left -= n, within = w1;
+        g.more = nt + AR_ITEM_COST - w1;
+        if (g.ends) within = 0, ++item;
         g.r0 = rb * R, g.n_rows = min(R, si.q_len * p.group - g.r0);
         const KeyRange kr = key_range(p, si, g.r0 / p.group, (g.r0 + g.n_rows - 1) / p.group + 1);
         g.t0 = max(g.st0, kr.a / AR_TILE), g.t1 = min(g.st1, (kr.b + AR_TILE - 1) / AR_TILE);
@@ -133,7 +141,7 @@ template <int R> struct ArTiles {  // tiles of all items of a sequence
     __device__ static __forceinline__ long count(const AttnParams& p, int s) {
         const SeqInfo si = seq_info(p, s);
         const KeyRange kr = key_range(p, si, 0, si.q_len);
-        return (long)((si.q_len * p.group + R - 1) / R) * p.nkv * max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - kr.a / AR_TILE);
+        return (long)((si.q_len * p.group + R - 1) / R) * p.nkv * (ar_tile_count(kr) + AR_ITEM_COST);
     }
 };
 template <int R> struct ArBlocks {  // row blocks of a sequence
@@ -141,8 +149,32 @@ template <int R> struct ArBlocks {  // row blocks of a sequence
 };
 // First tile of CTA c of n when `total` tiles are shared evenly
 __device__ __noinline__ long ar_share(long total, int c, int n) { return total * c / n; }
+// The last CTA of n whose share begins before place `end`
+__device__ __noinline__ int ar_last(long total, long end, int n) { return (int)((end * n + total - 1) / total) - 1; }
 constexpr int AR_MIN_TILES = 2;  // fewer tiles than this per CTA: fewer CTAs (a share of one tile costs more in joining than it saves)
 __device__ __forceinline__ int ar_ctas(long total, int grid) { return (int)max(1l, min((long)grid, total / AR_MIN_TILES)); }
+
+// The place of this CTA where up to 64 sequences are shared evenly, by one warp: each length is read once
+template <typename F>
+__device__ __noinline__ int plan_few(const AttnParams& p, long& total, int& n_ctas, long& share, long& before) {
+    const int lane = threadIdx.x & 31;
+    const long long c0 = lane < p.n_seqs ? (long long)F::count(p, lane) : 0ll, c1 = lane + 32 < p.n_seqs ? (long long)F::count(p, lane + 32) : 0ll;
+    long long i0 = c0, i1 = c1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u0 = __shfl_up_sync(0xffffffffu, i0, o), u1 = __shfl_up_sync(0xffffffffu, i1, o);
+        if (lane >= o) i0 += u0, i1 += u1;
+    }
+    i1 += __shfl_sync(0xffffffffu, i0, 31);
+    total = __shfl_sync(0xffffffffu, i1, 31);
+    n_ctas = ar_ctas(total, gridDim.x);
+    share = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
+    const unsigned p0 = __ballot_sync(0xffffffffu, i0 > share), p1 = __ballot_sync(0xffffffffu, i1 > share);
+    if (!(p0 | p1)) return -1;
+    const int f = __ffs(p0 ? p0 : p1) - 1;
+    before = __shfl_sync(0xffffffffu, p0 ? i0 - c0 : i1 - c1, f);
+    return p0 ? f : f + 32;
+}
 
 template <int HD, int R> struct ArScratch {  // layout of the scratch: joins, then per CTA two slots of (m, l) and outputs
     __host__ __device__ static size_t join_floats(int ctas) { return (size_t)ctas * (sizeof(ArJoin) / 4); }
@@ -179,34 +211,43 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
     pdl_wait_prior_grids();
     pdl_release_dependents();
 
-    int n_ctas = 1, first_seq;
-    long total = 0, before = 0, share = 0;  // tiles of the whole batch, before the sequence and before this CTA's share
-    if (p.stream_k) {
-        find_item<ArTiles<R>>(p, 1l << 62, total, hdr->scan);
-        n_ctas = ar_ctas(total, gridDim.x);
-        if (tid == 0) (reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x)->n_rows = 0;
-        if ((int)blockIdx.x >= n_ctas) return;
-        share = ar_share(total, blockIdx.x, n_ctas);
-        first_seq = find_item<ArTiles<R>>(p, share, before, hdr->scan);
-    } else {
-        first_seq = find_item<ArBlocks<R>>(p, blockIdx.y, before, hdr->scan);
+    // many sequences: all threads read their lengths; few: the copying warp alone
+    int n_ctas = 1, first_seq = 0;
+    long total = 0, before = 0, share = 0;  // places of the whole batch, before the sequence and before this CTA's share
+    if (p.n_seqs > AR_FEW_SEQS) {
+        if (p.stream_k) {
+            find_item<ArTiles<R>>(p, 1l << 62, total, hdr->scan);
+            n_ctas = ar_ctas(total, gridDim.x);
+            share = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
+            first_seq = find_item<ArTiles<R>>(p, share, before, hdr->scan);
+        } else {
+            first_seq = find_item<ArBlocks<R>>(p, blockIdx.y, before, hdr->scan);
+        }
     }
-    if (first_seq < 0) return;  // (no rows at all, or no such block)
-    __syncthreads();
     int it = 0;  // tiles so far, over all segments: stage it % STAGES
 
     if (warp == 4) {
         // ------------------------------------------------------------ plan and copies
         ArWalker<R> w{p};
-        w.s = first_seq;
-        w.load_seq();
-        if (p.stream_k) {
-            w.left = ar_share(total, blockIdx.x + 1, n_ctas) - share;
-            const int ahead = (int)(share - before);
-            w.item = ahead / w.nt, w.within = ahead - w.item * w.nt;
-        } else {  // one item per CTA: row block blockIdx.y of all (a sequence's last, longest, first), kv head blockIdx.x
-            w.left = w.nt, w.within = 0;
-            w.item = blockIdx.x * w.nrb + (w.nrb - 1 - (int)(blockIdx.y - before));
+        if (p.n_seqs <= AR_FEW_SEQS) {
+            if (p.stream_k) first_seq = plan_few<ArTiles<R>>(p, total, n_ctas, share, before);
+            else first_seq = warp_find_item<ArBlocks<R>>(p, blockIdx.y, before);
+        }
+        w.left = 0, w.s = first_seq, w.item = w.within = w.nrb = 0;
+        if (p.stream_k && lane == 0) {
+            (reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x)->n_rows = 0;
+            hdr->scan[34] = total, hdr->scan[35] = n_ctas;
+        }
+        if (first_seq >= 0 && (!p.stream_k || (int)blockIdx.x < n_ctas)) {  // else: nothing for this CTA
+            w.load_seq();
+            if (p.stream_k) {
+                w.left = ar_share(total, blockIdx.x + 1, n_ctas) - share;
+                const int ahead = (int)(share - before);
+                w.item = ahead / (w.nt + AR_ITEM_COST), w.within = ahead - w.item * (w.nt + AR_ITEM_COST);
+            } else {  // one item per CTA: row block blockIdx.y of all (a sequence's last, longest, first), kv head blockIdx.x
+                w.left = w.nt + AR_ITEM_COST, w.within = 0;
+                w.item = blockIdx.x * w.nrb + (w.nrb - 1 - (int)(blockIdx.y - before));
+            }
         }
         int q_no = 0;
         for (int n = 0; !*cta_abort; ++n) {
@@ -432,7 +473,7 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
                 if (!whole && lane == 0) sml[2 * r] = em, sml[2 * r + 1] = el;
             }
         } else if constexpr (WM == 1) {
-            // the four warps' parts, added in warp order through one buffer
+            // the four warps' parts, added through one buffer in a fixed order
             if (pq == 0)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) hdr->ml[warp][qr + 8 * e][0] = m[e], hdr->ml[warp][qr + 8 * e][1] = l[e];
@@ -444,18 +485,21 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
                 const float mm = fmaxf(fmaxf(hdr->ml[0][r][0], hdr->ml[1][r][0]), fmaxf(hdr->ml[2][r][0], hdr->ml[3][r][0]));
                 f[e] = m[e] == -INFINITY ? 0.f : fast_exp2((m[e] - mm) * p.scale_log2);
             }
+#pragma unroll 1
             for (int u = 0; u < 4; ++u) {
                 if (warp == u) {
 #pragma unroll
-                    for (int n = 0; n < HD / 8; ++n)
+                    for (int e = 0; e < 2; ++e) {
+                        if (qr + 8 * e >= n_rows) continue;
+                        float* row = buf + (qr + 8 * e) * Sh::BUF_PITCH + 2 * pq;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float2* d = reinterpret_cast<float2*>(buf + (qr + 8 * e) * Sh::BUF_PITCH + 8 * n + 2 * pq);
-                            float2 x = u == 0 ? make_float2(0.f, 0.f) : *d;
+                        for (int i = 0; i < HD / 8; ++i) {
+                            float2* d = reinterpret_cast<float2*>(row + 8 * i);
+                            const float2 x = u == 0 ? make_float2(0.f, 0.f) : *d;
                             // (a warp without keys has zeros, which a factor of 0 keeps; one with a NaN keeps that too)
-                            x.x += o[n][2 * e] * f[e], x.y += o[n][2 * e + 1] * f[e];
-                            *d = x;
+                            *d = make_float2(x.x + o[i][2 * e] * f[e], x.y + o[i][2 * e + 1] * f[e]);
                         }
+                    }
                 }
                 math_sync();
             }
@@ -497,10 +541,10 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
             ArJoin j;
             j.s = w.s, j.q0 = w.q0, j.tok_row0 = r0, j.n_rows = n_rows, j.kvh = w.kvh;
             j.any_key = pos0;  // position of token 0
+            const long total = hdr->scan[34];
+            const int n_ctas = (int)hdr->scan[35];
             const long item_end = ar_share(total, blockIdx.x + 1, n_ctas) + w.more;  // (a segment that does not end its item ends the share)
-            int c = blockIdx.x + 1;
-            while (ar_share(total, c + 1, n_ctas) < item_end) ++c;
-            j.n_parts = c - (int)blockIdx.x + 1, j.pad = 0;
+            j.n_parts = ar_last(total, item_end, n_ctas) - (int)blockIdx.x + 1, j.pad = 0;
             reinterpret_cast<ArJoin*>(p.scratch)[blockIdx.x] = j;
         }
         __syncwarp();
@@ -508,48 +552,77 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
     }
 }
 
-// Adds the parts of the items that several CTAs share, in key order.  A warp per row.
+// Adds the parts of the items that several CTAs share, in key order.  A warp per row, eight parts in flight (one after the other,
+// each took a round trip to L2: 10 us for 37 parts).
 template <int HD, int R>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnParams p, int ctas) {
+    constexpr int E = HD / 32, BATCH = 8;  // elements of a lane: E lane .. E lane + E - 1
     pdl_wait_prior_grids();
     const ArJoin j = reinterpret_cast<const ArJoin*>(p.scratch)[blockIdx.x];
     const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (r >= j.n_rows) return;
-    const int c0 = blockIdx.x;
-    auto slot_of = [&](int i) { return 2 * (c0 + i) + (i == 0 ? 1 : 0); };
+    auto slot_of = [&](int i) { return 2 * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0); };
+    auto load = [&](int i, float (&x)[E]) {
+        const float* o = ArScratch<HD, R>::o(p.scratch, ctas, slot_of(i)) + (size_t)r * HD + E * lane;
+        if constexpr (E % 4 == 0) {
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(o + e);
+                x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
+            }
+        } else if constexpr (E == 2) {
+            const float2 v = *reinterpret_cast<const float2*>(o);
+            x[0] = v.x, x[1] = v.y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = o[e];
+        }
+    };
+    float x[BATCH][E];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+        if (i < j.n_parts) load(i, x[i]);
     float mm = -INFINITY;
     for (int i = lane; i < j.n_parts; i += 32) mm = fmaxf(mm, ArScratch<HD, R>::ml(p.scratch, ctas, slot_of(i))[2 * r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
     const float mu = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, acc[HD / 32];
+    float ll = 0.f, acc[E];
 #pragma unroll
-    for (int e = 0; e < HD / 32; ++e) acc[e] = 0.f;
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
     for (int i0 = 0; i0 < j.n_parts; i0 += 32) {
         float f = 0.f, lp = 0.f;
         if (i0 + lane < j.n_parts) {
             const float* ml = ArScratch<HD, R>::ml(p.scratch, ctas, slot_of(i0 + lane)) + 2 * r;
-            f = fast_exp2((ml[0] - mu) * p.scale_log2);
-            // (a part without keys: maximum -inf, sum 0; its factor of 0 keeps both)
+            f = fast_exp2((ml[0] - mu) * p.scale_log2);  // (a part without keys: maximum -inf, sum 0; its factor of 0 keeps both)
             lp = ml[1] * f;
-            if (ml[1] != ml[1]) lp = ml[1];
         }
         const int n = min(32, j.n_parts - i0);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-            const float fi = __shfl_sync(0xffffffffu, f, i);
-            ll += __shfl_sync(0xffffffffu, lp, i);
-            const float* o = ArScratch<HD, R>::o(p.scratch, ctas, slot_of(i0 + i)) + (size_t)r * HD;
+        for (int b = 0; b < n; b += BATCH) {
+            float y[BATCH][E];
 #pragma unroll
-            for (int e = 0; e < HD / 32; ++e) acc[e] += o[lane + 32 * e] * fi;
+            for (int i = 0; i < BATCH; ++i) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[i][e] = x[i][e];
+                if (i0 + b + BATCH + i < j.n_parts) load(i0 + b + BATCH + i, x[i]);  // the next batch
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const float fi = __shfl_sync(0xffffffffu, f, b + i), li = __shfl_sync(0xffffffffu, lp, b + i);
+                if (b + i < n) {
+                    ll += li;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += y[i][e] * fi;
+                }
+            }
         }
     }
     const int tok = (j.tok_row0 + r) / p.group, h = j.kvh * p.group + (j.tok_row0 + r) % p.group;
     const bool sees = j.any_key + tok >= 0;
     const float inv = 1.f / ll;
 #pragma unroll
-    for (int e = 0; e < HD / 32; ++e)
-        store_out1(p.out, p.out_dtype, (size_t)(j.q0 + tok) * p.out_stride + (size_t)h * HD + lane + 32 * e, sees ? acc[e] * inv : 0.f);
+    for (int e = 0; e < E; ++e)
+        store_out1(p.out, p.out_dtype, (size_t)(j.q0 + tok) * p.out_stride + (size_t)h * HD + E * lane + e, sees ? acc[e] * inv : 0.f);
 }
 
 // ---- host side ----

@@ -187,42 +187,19 @@ __device__ __forceinline__ int at_tile_count(const KeyRange& kr) { return max(1,
 struct AtItems {  // items of a sequence
     __device__ static __forceinline__ int count(const AttnParams& p, int s) { return (seq_info(p, s).q_len + at_block_tokens(p) - 1) / at_block_tokens(p) * p.nkv; }
 };
+constexpr int AT_ITEM_COST = 2;
 struct AtTiles {  // tiles of them all
     __device__ static __forceinline__ long count(const AttnParams& p, int s) {
         const SeqInfo si = seq_info(p, s);
-        return (long)((si.q_len + at_block_tokens(p) - 1) / at_block_tokens(p)) * p.nkv * at_tile_count(key_range(p, si, 0, si.q_len));
+        return (long)((si.q_len + at_block_tokens(p) - 1) / at_block_tokens(p)) * p.nkv * (at_tile_count(key_range(p, si, 0, si.q_len)) + AT_ITEM_COST);
     }
 };
-
-// As find_item, by one warp: 32 sequences at a time
-template <typename F>
-__device__ __noinline__ int warp_find_item(const AttnParams& p, long target, long& before) {
-    const int lane = threadIdx.x & 31;
-    before = 0;
-#pragma unroll 1
-    for (int base = 0; base < p.n_seqs; base += 32) {
-        const long long cnt = base + lane < p.n_seqs ? (long long)F::count(p, base + lane) : 0ll;
-        long long inc = cnt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, before + inc > target);
-        if (past) {
-            const int f = __ffs(past) - 1;
-            before += __shfl_sync(0xffffffffu, inc - cnt, f);
-            return base + f;
-        }
-        before += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    return -1;
-}
 
 // The segments of this CTA, walked by the planning warp.  An item is (sequence, kv head, block of tb tokens).
 // Many items: whole items, CTA c of n takes number c, 2n-1-c, 2n+c, ... of all (a sequence's last, longest blocks first, every
 // second round backwards: the rounds' differences cancel).  Few items over a long axis (stream_k): all tiles are shared evenly in
-// order, where every item of a sequence counts as many tiles as its last block has, at least one.
+// order, where every item of a sequence counts as many tiles as its last block has, at least one, and AT_ITEM_COST more (as in
+// ArWalker).
 struct AtWalker {
     const AttnParams& p;
     int tb;        // tokens per block
@@ -278,13 +255,15 @@ struct AtWalker {
                 item = within = 0;
                 load_seq();
             }
-            const int n = min(left, nt - within);
+            if (within == 0 && left <= AT_ITEM_COST) return false;  // (its first places: the item is the next CTA's)
+            if (within > 0 && within <= AT_ITEM_COST) left += within, within = 0;
+            const int n = min(left, nt + AT_ITEM_COST - within), w1 = within + n;
             g.kvh = item / nb, blk = item - g.kvh * nb;
-            g.st0 = tl + within, g.st1 = g.st0 + n;
-            g.begins = within == 0, g.ends = within + n == nt;
-            left -= n, within += n;
-            g.more = nt - within;
-            if (within == nt) within = 0, ++item;
+            g.begins = within == 0, g.ends = w1 == nt + AT_ITEM_COST;
+            g.st0 = tl + max(0, within - AT_ITEM_COST), g.st1 = tl + w1 - AT_ITEM_COST;
+            left -= n, within = w1;
+            g.more = nt + AT_ITEM_COST - w1;
+            if (g.ends) within = 0, ++item;
         } else {
             if (!skip(ahead)) return false;
             const int n = gridDim.x, c = blockIdx.x;
@@ -392,11 +371,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         AtWalker w{p, 2 * tpt};
         bool any = true;
         if (p.stream_k) {
-            if (p.n_seqs <= AT_FEW_SEQS) {
-                warp_find_item<AtTiles>(p, 1l << 62, total);
-                n_ctas = ar_ctas(total, gridDim.x), share = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
-                first_seq = warp_find_item<AtTiles>(p, share, before);
-            }
+            if (p.n_seqs <= AT_FEW_SEQS) first_seq = plan_few<AtTiles>(p, total, n_ctas, share, before);
             if (lane == 0) {
                 (reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x)->n_rows = 0;
                 hdr->scan[34] = total, hdr->scan[35] = n_ctas;
@@ -406,7 +381,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 w.left = (int)(ar_share(total, blockIdx.x + 1, n_ctas) - share), w.s = first_seq;
                 w.load_seq();
                 const int ahead = (int)(share - before);  // (a sequence's tiles fit 31 bits: the entry point checks)
-                w.item = ahead / w.nt, w.within = ahead - w.item * w.nt;
+                w.item = ahead / (w.nt + AT_ITEM_COST), w.within = ahead - w.item * (w.nt + AT_ITEM_COST);
             }
         } else {
             w.s = first_seq, w.item = w.nb = w.within = 0, w.left = 1, w.ahead = blockIdx.x, w.turn = 0;
@@ -787,9 +762,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 const long total = hdr->scan[34];
                 const int n_ctas = (int)hdr->scan[35];
                 const long item_end = ar_share(total, blockIdx.x + 1, n_ctas) + w.more;  // (a segment that does not end its item ends the share)
-                int e = blockIdx.x + 1;
-                while (ar_share(total, e + 1, n_ctas) < item_end) ++e;
-                j.n_parts = e - (int)blockIdx.x + 1, j.pad = 0;
+                j.n_parts = ar_last(total, item_end, n_ctas) - (int)blockIdx.x + 1, j.pad = 0;
                 reinterpret_cast<ArJoin*>(p.scratch)[blockIdx.x] = j;
             }
         }
