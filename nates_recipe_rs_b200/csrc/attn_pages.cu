@@ -1,6 +1,7 @@
 // Entry points of the operators on a paged KV cache and on packed prompts (declared in include/qmm.h): argument checks, tensor
 // maps and the choice of kernel.
 #include "attn_pages.cuh"
+#include <algorithm>
 #include <cmath>
 
 namespace qmm {
@@ -74,6 +75,7 @@ static int attn_run_form(AttnForm form, AttnParams& p, int dtype, int hd, long r
     const int box = p.table ? gcd_int(p.page_size, tile) : tile;  // pages are multiples of 8, tiles powers of two
     for (p.box_shift = 3; 1 << p.box_shift < box;) ++p.box_shift;
     p.group_inv = (65536 + p.group - 1) / p.group;
+    p.row_tiles = attn_tiles_rows(hd) / 128;
     CUtensorMap km, vm;
     if (int st = kv_tensor_map(&km, p.k, dtype, hd, p.nkv, rows, n_pages, p.k_row, p.k_page, box)) return st;
     if (int st = kv_tensor_map(&vm, p.v, dtype, hd, p.nkv, rows, n_pages, p.v_row, p.v_page, box)) return st;
@@ -114,10 +116,12 @@ int launch_rope_kv_append_paged(const void* qkv, int qkv_dtype, long qkv_stride,
     for (int j = 1; j < p.half; ++j) p.freq[j] = p.freq[j - 1] * step;
     // 16-byte accesses where every head, half head and row begins on one
     const bool wide = p.half % 8 == 0 && hd % 8 == 0 && !misaligned(qkv, 16) && !misaligned(q_out, 16) && qkv_stride * size_in % 16 == 0;
-    // enough tokens per CTA that its threads have two units of work each, as long as every SM keeps several CTAs
-    const long units = (long)(n_q_heads + 2 * nkv) * hd / 16;
-    p.tokens = 1;
-    while (p.tokens < KVA_MAX_TOKENS && p.tokens * units < 2 * KVA_THREADS && seqs->total_q / (2 * p.tokens) >= 8 * sm_count()) p.tokens *= 2;
+    // As few CTAs as run at once (six per SM), so that what a CTA does before its first byte (finding the sequences, the angles) is
+    // not paid in two rounds: 2431 tokens of 20 heads of 96 take 7.6 us with three tokens per CTA, 11.2 with one; but no more work
+    // than twice what its threads take at a time, or two tokens: 12122 tokens of 80 heads of 128 take 121 us with two, 131 with eight
+    const long units = (long)(n_q_heads + 2 * nkv) * hd / 16, at_once = 6l * sm_count();
+    const long most = std::min<long>(KVA_MAX_TOKENS, std::max<long>(2, 2 * KVA_THREADS / std::max<long>(units, 1)));
+    p.tokens = (int)std::min(most, std::max<long>(1, (seqs->total_q + at_once - 1) / at_once));
     cudaStream_t s = as_stream(stream);
     const bool f16 = kv->dtype == QMM_DT_F16;
     if (qkv_dtype == QMM_DT_F32) return f16 ? kv_append_inst<float, __half>(p, wide, s) : kv_append_inst<float, __nv_bfloat16>(p, wide, s);
@@ -155,7 +159,7 @@ int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, cons
     p.scale_log2 = kq_scale * 1.4426950408889634f;
     // decode, and more rows where their items would not fill the GPU several times over: the tiles are shared evenly
     const AttnForm form = attn_form(seqs->max_q, p.group, hd);
-    const long items = ((long)p.total_q * p.group / (form == ATTN_TILES ? AT_MAX_ROWS : 64) + 1) * nkv;
+    const long items = ((long)p.total_q * p.group / (form == ATTN_TILES ? attn_tiles_rows(hd) : 64) + 1) * nkv;
     p.stream_k = form == ATTN_NARROW || items < 4l * sm_count();
     return attn_run_form(form, p, kv->dtype, hd, p.page_size, p.n_pages, as_stream(stream));
 }

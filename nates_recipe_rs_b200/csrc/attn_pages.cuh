@@ -29,6 +29,7 @@ struct AttnParams {
     int n_seqs, total_q, max_kv;
     int nqh, nkv, group, window, out_dtype;
     int box_shift;                           // rows of one tensor-map box: 1 << box_shift, divides the tile and the page
+    int row_tiles;                           // attn_tiles.cu: tiles of 128 rows of an item
     int group_inv;                           // ceil(2^16 / group): r / group = r * group_inv >> 16 for the rows r < 256 of an item
     int stream_k;                            // 1: the CTAs share all (item, tile) pairs evenly and joined items go through scratch
     float scale_log2;                        // kq_scale * log2(e)
@@ -213,16 +214,16 @@ __device__ __forceinline__ void tile_boxes(const AttnParams& p, int t, int a, in
     first = lo >> p.box_shift;
     count = hi > lo ? ((hi - 1) >> p.box_shift) - first + 1 : 0;
 }
-// Issued by a whole warp: the boxes of one matrix's tile.  `pages` holds, in lane j, the page of box j (page_of_boxes).
+// Issued by a whole warp: the boxes of one matrix's tile, elements from x0 on.  `pages` holds, in lane j, the page of box j (page_of_boxes).
 template <int TILE, int NCH>
-__device__ __forceinline__ void load_tile(const AttnParams& p, const CUtensorMap* map, uint32_t dst, uint32_t bar, int t, int first, int count,
+__device__ __forceinline__ void load_tile(const AttnParams& p, const CUtensorMap* map, uint32_t dst, uint32_t bar, int x0, int first, int count,
                                           int pages, int slots, int kvh) {
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
     for (int i = lane; i - lane < count * NCH; i += 32) {  // (the whole warp stays in the loop: the shuffles need it)
         const int j = first + i / NCH, c = i % NCH;
         const int pg = __shfl_sync(0xffffffffu, pages, j & 31), slot = __shfl_sync(0xffffffffu, slots, j & 31);
-        if (i < count * NCH) tma_load_4d(dst + (uint32_t)(c * TILE + (j << p.box_shift)) * 128u, map, c * 64, kvh, slot, pg, bar);
+        if (i < count * NCH) tma_load_4d(dst + (uint32_t)(c * TILE + (j << p.box_shift)) * 128u, map, x0 + c * 64, kvh, slot, pg, bar);
     }
 }
 // lane j: page and slot of the first position of box j of tile t (looked up ahead of the tile's turn); packed rows are one page

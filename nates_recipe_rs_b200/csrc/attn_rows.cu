@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
             w.load_seq();
             if (p.stream_k) {
                 w.left = ar_share(total, blockIdx.x + 1, n_ctas) - share;
-                const int ahead = (int)(share - before);
-                w.item = ahead / (w.nt + AR_ITEM_COST), w.within = ahead - w.item * (w.nt + AR_ITEM_COST);
+                const long ahead = share - before;
+                w.item = (int)(ahead / (w.nt + AR_ITEM_COST)), w.within = (int)(ahead - (long)w.item * (w.nt + AR_ITEM_COST));
             } else {  // one item per CTA: row block blockIdx.y of all (a sequence's last, longest, first), kv head blockIdx.x
                 w.left = w.nt + AR_ITEM_COST, w.within = 0;
                 w.item = blockIdx.x * w.nrb + (w.nrb - 1 - (int)(blockIdx.y - before));
@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
                 const uint32_t bar = smem_u32(&hdr->full[st]), dst = ring + (uint32_t)st * 2 * Sh::TILE_BYTES;
                 if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(count * 2 * Sh::NCH * 128) << p.box_shift);
                 __syncwarp();
-                load_tile<AR_TILE, Sh::NCH>(p, &kmap, dst, bar, t, first, count, pages, slots, g.kvh);
-                load_tile<AR_TILE, Sh::NCH>(p, &vmap, dst + Sh::TILE_BYTES, bar, t, first, count, pages, slots, g.kvh);
+                load_tile<AR_TILE, Sh::NCH>(p, &kmap, dst, bar, 0, first, count, pages, slots, g.kvh);
+                load_tile<AR_TILE, Sh::NCH>(p, &vmap, dst + Sh::TILE_BYTES, bar, 0, first, count, pages, slots, g.kvh);
                 first = nfirst, count = ncount, pages = npages, slots = nslots;
             }
         }
@@ -657,12 +657,12 @@ static long attn_rows_scratch_bytes(int hd, bool narrow) {
     case 64: return ar_scratch_bytes_of<64, 1>();
     case 96: return ar_scratch_bytes_of<96, 1>();
     case 128: return ar_scratch_bytes_of<128, 1>();
-    case 256: return narrow ? ar_scratch_bytes_of<256, 1>() : ar_scratch_bytes_of<256, 4>();
+    case 256: return ar_scratch_bytes_of<256, 1>();
     }
     return QMM_ERR_UNSUPPORTED;
 }
 
-// narrow: up to 16 rows per item; otherwise (head_dim 32 and 256 only: the others have attn_tiles.cu) 64
+// narrow: up to 16 rows per item; otherwise (head_dim 32 only: the others have attn_tiles.cu) 64
 static int attn_rows_launch(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, int dtype, int hd, bool narrow, cudaStream_t s) {
     const bool f16 = dtype == QMM_DT_F16;
 #define QMM_AR_CASE(HD_, WM_) return f16 ? attn_rows_inst<__half, HD_, WM_>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, HD_, WM_>(p, km, vm, s)
@@ -673,9 +673,7 @@ static int attn_rows_launch(const AttnParams& p, const CUtensorMap& km, const CU
     case 64: QMM_AR_CASE(64, 1);
     case 96: QMM_AR_CASE(96, 1);
     case 128: QMM_AR_CASE(128, 1);
-    case 256:
-        if (narrow) QMM_AR_CASE(256, 1);
-        QMM_AR_CASE(256, 4);
+    case 256: QMM_AR_CASE(256, 1);
     }
 #undef QMM_AR_CASE
     return QMM_ERR_UNSUPPORTED;

@@ -27,17 +27,20 @@
 namespace qmm {
 
 constexpr int AT_TILE = 128;  // keys per tile, and rows per tile
-constexpr int AT_THREADS = 640;  // 16 softmax warps, two issuing warps, the copying and the planning warp (a 21st would leave 80 registers)
-constexpr int AT_WARP_MMA0 = 16, AT_WARP_COPY = 17, AT_WARP_PLAN = 18, AT_WARP_MMA1 = 19;
 constexpr int AT_SEGS = 4;  // segments planned ahead
 constexpr int AT_FEW_SEQS = 64;  // up to this many sequences the planning warp finds its place alone, beyond the whole CTA does
-constexpr int AT_MAX_ROWS = 256;  // rows of an item
 template <int HD> struct AtShape {
-    static constexpr int NCH = (HD + 63) / 64;
-    static constexpr int TILE_BYTES = NCH * AT_TILE * 128;  // 128 rows of one matrix
-    static constexpr int SLOTS = NCH == 1 ? 10 : 5;         // 160 KB of keys and values
+    static constexpr bool WIDE = HD > 128;            // one row tile, its scores in two buffers
+    static constexpr int HALVES = WIDE ? 2 : 1;       // slots of a tile of keys (or values): 128 keys x up to 128 elements each
+    static constexpr int NCH = (HD / HALVES + 63) / 64;  // chunks of 64 elements of a slot
+    static constexpr int TILE_BYTES = NCH * AT_TILE * 128;
+    static constexpr int SLOTS = NCH == 1 ? 10 : 5;   // 160 KB of keys and values
+    static constexpr int ROW_TILES = WIDE ? 1 : 2, MAX_ROWS = 128 * ROW_TILES;
+    // warps: softmax (eight per row tile), issuing, copying, planning, issuing for the second row tile; 20 (a 21st would leave 80 registers)
+    static constexpr int SOFTMAX = 8 * ROW_TILES, MMA0 = SOFTMAX, COPY = SOFTMAX + 1, PLAN = SOFTMAX + 2, MMA1 = SOFTMAX + 3;
+    static constexpr int WARPS = SOFTMAX + 2 + ROW_TILES, THREADS = 32 * WARPS;
     __host__ __device__ static constexpr uint32_t IDESC_S(bool bf16) { return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((AT_TILE >> 3) << 17) | ((128 >> 4) << 24); }
-    __host__ __device__ static constexpr uint32_t IDESC_O(bool bf16) { return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24); }
+    __host__ __device__ static constexpr uint32_t IDESC_O(bool bf16) { return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((HD / HALVES >> 3) << 17) | ((128 >> 4) << 24); }
 };
 // tensor memory columns: S of tile i at 128 i, P over the second half of S (the half that is read last goes there first), O of
 // tile i at 256 + 128 i
@@ -182,7 +185,7 @@ __device__ __forceinline__ void exp64(const uint32_t (&s)[32], float c, const fl
     tmem_st_p(tp, pk);
 }
 
-__device__ __forceinline__ int at_block_tokens(const AttnParams& p) { return 2 * (AT_TILE * p.group_inv >> 16); }  // of an item
+__device__ __forceinline__ int at_block_tokens(const AttnParams& p) { return p.row_tiles * (AT_TILE * p.group_inv >> 16); }  // of an item
 __device__ __forceinline__ int at_tile_count(const KeyRange& kr) { return max(1, (max(kr.b, 0) + AT_TILE - 1) / AT_TILE - kr.a / AT_TILE); }
 struct AtItems {  // items of a sequence
     __device__ static __forceinline__ int count(const AttnParams& p, int s) { return (seq_info(p, s).q_len + at_block_tokens(p) - 1) / at_block_tokens(p) * p.nkv; }
@@ -203,7 +206,7 @@ struct AtTiles {  // tiles of them all
 struct AtWalker {
     const AttnParams& p;
     int tb;        // tokens per block
-    int left;      // stream_k: tiles of this CTA's share still to come; else 0 after the last item
+    long left;     // stream_k: places of this CTA's share still to come
     int ahead, turn;  // items from the current one to the next, rounds so far
     int s, item, within;
     SeqInfo si;
@@ -257,7 +260,7 @@ struct AtWalker {
             }
             if (within == 0 && left <= AT_ITEM_COST) return false;  // (its first places: the item is the next CTA's)
             if (within > 0 && within <= AT_ITEM_COST) left += within, within = 0;
-            const int n = min(left, nt + AT_ITEM_COST - within), w1 = within + n;
+            const int n = (int)min(left, (long)(nt + AT_ITEM_COST - within)), w1 = within + n;
             g.kvh = item / nb, blk = item - g.kvh * nb;
             g.begins = within == 0, g.ends = w1 == nt + AT_ITEM_COST;
             g.st0 = tl + max(0, within - AT_ITEM_COST), g.st1 = tl + w1 - AT_ITEM_COST;
@@ -306,7 +309,7 @@ __device__ __noinline__ void at_exact_rows(const AttnParams& p, const AtSeg& w, 
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                                                                    const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams params) {
     using Sh = AtShape<HD>;
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -320,10 +323,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
     const int tpt = AT_TILE / params.group, tile_rows = tpt * params.group;  // tokens and rows of a row tile
 
     if (tid == 0) {
-        for (int i = 0; i < Sh::SLOTS; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), 2);
-        mbar_init(smem_u32(&hdr->v_ask), 2), mbar_init(smem_u32(&hdr->v_ok), 1);
-        mbar_init(smem_u32(&hdr->q_full), 1), mbar_init(smem_u32(&hdr->q_empty), 2);
-        for (int i = 0; i < AT_SEGS; ++i) mbar_init(smem_u32(&hdr->seg_full[i]), 1), mbar_init(smem_u32(&hdr->seg_empty[i]), 19);
+        constexpr int N = Sh::ROW_TILES;  // issuing threads
+        for (int i = 0; i < Sh::SLOTS; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), N);
+        mbar_init(smem_u32(&hdr->v_ask), N), mbar_init(smem_u32(&hdr->v_ok), 1);
+        mbar_init(smem_u32(&hdr->q_full), 1), mbar_init(smem_u32(&hdr->q_empty), N);
+        for (int i = 0; i < AT_SEGS; ++i) mbar_init(smem_u32(&hdr->seg_full[i]), 1), mbar_init(smem_u32(&hdr->seg_empty[i]), Sh::WARPS - 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&hdr->s_full[i]), 1), mbar_init(smem_u32(&hdr->o_full[i]), 1), mbar_init(smem_u32(&hdr->drain[i]), 1);
             mbar_init(smem_u32(&hdr->p_part[i]), 8), mbar_init(smem_u32(&hdr->p_full[i]), 8);
@@ -332,7 +336,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         hdr->abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == AT_WARP_MMA0) {
+    if (warp == Sh::MMA0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&hdr->tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -366,9 +370,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         if (lane == 0) mbar_arrive(smem_u32(&hdr->seg_empty[n % AT_SEGS]));
     };
 
-    if (warp == AT_WARP_PLAN) {
+    if (warp == Sh::PLAN) {
         // ------------------------------------------------------------ plan: the only code that knows how items follow one another
-        AtWalker w{p, 2 * tpt};
+        AtWalker w{p, Sh::ROW_TILES * tpt};
         bool any = true;
         if (p.stream_k) {
             if (p.n_seqs <= AT_FEW_SEQS) first_seq = plan_few<AtTiles>(p, total, n_ctas, share, before);
@@ -378,10 +382,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
             }
             any = (int)blockIdx.x < n_ctas && first_seq >= 0;
             if (any) {
-                w.left = (int)(ar_share(total, blockIdx.x + 1, n_ctas) - share), w.s = first_seq;
+                w.left = ar_share(total, blockIdx.x + 1, n_ctas) - share, w.s = first_seq;
                 w.load_seq();
-                const int ahead = (int)(share - before);  // (a sequence's tiles fit 31 bits: the entry point checks)
-                w.item = ahead / (w.nt + AT_ITEM_COST), w.within = ahead - w.item * (w.nt + AT_ITEM_COST);
+                const long ahead = share - before;
+                w.item = (int)(ahead / (w.nt + AT_ITEM_COST)), w.within = (int)(ahead - (long)w.item * (w.nt + AT_ITEM_COST));
             }
         } else {
             w.s = first_seq, w.item = w.nb = w.within = 0, w.left = 1, w.ahead = blockIdx.x, w.turn = 0;
@@ -416,29 +420,31 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                 mbar_arrive(smem_u32(&hdr->seg_full[n % AT_SEGS]));
             }
             __syncwarp();
-            for (int t = last.t0; t < last.t1; ++t, it += 2) {
+            const int tiles = max(last.t1 - last.t0, 0);
+            for (int k = 0; k < tiles; ++k) {
+                const int t = last.t0 + k;
                 if (!last.dirty(t)) continue;
-                const int sl = (it + 1) % Sh::SLOTS;
                 if (!wait(&hdr->v_ask, n_v++, DEV_TIMEOUT_FULL)) {
                     ok = false;
                     break;
                 }
-                uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)(2 + sl) * Sh::TILE_BYTES);
                 const int c0 = min(max(((last.a >> p.box_shift) << p.box_shift) - t * AT_TILE, 0), AT_TILE), c1 = max(min(last.kv - t * AT_TILE, AT_TILE), c0);
+                // order of the slots: K0 V0 K1 V1 ..., or (scores one tile ahead) K0 K1 V0 K2 V1 ...
+                const int v_it = it + (Sh::WIDE ? 2 * (min(k + 2, tiles) + k) : 2 * k + 1);
 #pragma unroll 1
-                for (int ch = 0; ch < Sh::NCH; ++ch) {
-                    for (int i = lane; i < c0 * 8; i += 32) vp[ch * AT_TILE * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
-                    for (int i = c1 * 8 + lane; i < AT_TILE * 8; i += 32) vp[ch * AT_TILE * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
+                for (int ch = 0; ch < Sh::NCH * Sh::HALVES; ++ch) {
+                    uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)(2 + (v_it + ch / Sh::NCH) % Sh::SLOTS) * Sh::TILE_BYTES) + (ch % Sh::NCH) * AT_TILE * 8;
+                    for (int i = lane; i < c0 * 8; i += 32) vp[i] = make_uint4(0u, 0u, 0u, 0u);
+                    for (int i = c1 * 8 + lane; i < AT_TILE * 8; i += 32) vp[i] = make_uint4(0u, 0u, 0u, 0u);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read by the tensor cores, refilled by a copy
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ok));
             }
+            it += 2 * Sh::HALVES * tiles;
             last = g;
         }
-    } else
-
-    if (warp == AT_WARP_COPY) {
+    } else if (warp == Sh::COPY) {
         // ------------------------------------------------------------ copies
         int it = 0, q_no = 0;  // tiles (of keys and of values) and query blocks so far
         bool ok = true;
@@ -446,37 +452,44 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
             const AtSeg& w = hdr->seg[n % AT_SEGS];
             const int t0 = w.t0, t1 = w.t1, kvh = w.kvh, q0 = w.q0, kv_len = w.kv;
             if (t0 >= t1) continue;
-            const int nq = w.tok1 - w.tok0 > tpt ? 2 : 1;
+            const int nq = Sh::WIDE || w.tok1 - w.tok0 > tpt ? 2 : 1;
             int first, cnt, pages, slots;
             tile_boxes<AT_TILE>(p, t0, w.a, kv_len, first, cnt);
             pages = page_of_boxes<AT_TILE>(p, w.s, q0, t0, first, cnt, slots);
             if (q_no > 0 && !wait(&hdr->q_empty, q_no - 1, DEV_TIMEOUT_EMPTY)) break;
             if (lane == 0) mbar_arrive_expect_tx(smem_u32(&hdr->q_full), (uint32_t)(nq * Sh::NCH * tile_rows * 128));
             __syncwarp();
-            if (lane < nq * Sh::NCH) {
+            if (lane < nq * Sh::NCH) {  // (nq: row tiles, or halves of the elements)
                 const int i = lane / Sh::NCH, c = lane % Sh::NCH;
-                tma_load_3d(q_s + (uint32_t)(i * Sh::TILE_BYTES + c * AT_TILE * 128), &qmap, c * 64, kvh * p.group, q0 + w.tok0 + i * tpt,
-                            smem_u32(&hdr->q_full));
+                tma_load_3d(q_s + (uint32_t)(i * Sh::TILE_BYTES + c * AT_TILE * 128), &qmap, (Sh::WIDE ? lane : c) * 64, kvh * p.group,
+                            q0 + w.tok0 + (Sh::WIDE ? 0 : i * tpt), smem_u32(&hdr->q_full));
             }
             ++q_no;
+            auto load = [&](const CUtensorMap* map, int t, int first, int cnt, int pages, int slots) {
+#pragma unroll 1
+                for (int h = 0; h < Sh::HALVES; ++h, ++it) {
+                    const int sl = it % Sh::SLOTS;
+                    if (it >= Sh::SLOTS && !wait(&hdr->empty[sl], it / Sh::SLOTS - 1, DEV_TIMEOUT_EMPTY)) return false;
+                    const uint32_t bar = smem_u32(&hdr->full[sl]);
+                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(cnt * Sh::NCH * 128) << p.box_shift);
+                    __syncwarp();
+                    load_tile<AT_TILE, Sh::NCH>(p, map, ring + (uint32_t)sl * Sh::TILE_BYTES, bar, h * 128, first, cnt, pages, slots, kvh);
+                }
+                return true;
+            };
             for (int t = t0; t < t1 && ok; ++t) {
                 int nfirst = 0, ncnt = 0, npages = 0, nslots = 0;
                 if (t + 1 < t1) {  // the next tile's pages are looked up before its turn comes
                     tile_boxes<AT_TILE>(p, t + 1, w.a, kv_len, nfirst, ncnt);
                     npages = page_of_boxes<AT_TILE>(p, w.s, q0, t + 1, nfirst, ncnt, nslots);
                 }
-#pragma unroll 1
-                for (int kv = 0; kv < 2; ++kv, ++it) {
-                    const int sl = it % Sh::SLOTS;
-                    if (it >= Sh::SLOTS && !wait(&hdr->empty[sl], it / Sh::SLOTS - 1, DEV_TIMEOUT_EMPTY)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t bar = smem_u32(&hdr->full[sl]);
-                    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(cnt * Sh::NCH * 128) << p.box_shift);
-                    __syncwarp();
-                    load_tile<AT_TILE, Sh::NCH>(p, kv ? &vmap : &kmap, ring + (uint32_t)sl * Sh::TILE_BYTES, bar, t, first, cnt, pages, slots, kvh);
+                if (Sh::WIDE) {
+                    if (t == t0) ok = load(&kmap, t, first, cnt, pages, slots);
+                    if (ok && t + 1 < t1) ok = load(&kmap, t + 1, nfirst, ncnt, npages, nslots);
+                } else {
+                    ok = load(&kmap, t, first, cnt, pages, slots);
                 }
+                ok = ok && load(&vmap, t, first, cnt, pages, slots);
                 first = nfirst, cnt = ncnt, pages = npages, slots = nslots;
             }
         }
@@ -494,11 +507,92 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                     }
             }
         }
-    } else if (warp == AT_WARP_MMA0 || warp == AT_WARP_MMA1) {
+    } else if (Sh::WIDE && warp == Sh::MMA0) {
+        // ------------------------------------------------------------ tensor cores, wide heads: scores one tile ahead of the outputs
+        // (one row tile, so its scores have two buffers and the next ones are ready when a softmax ends)
+        int it = 0, q_no = 0;
+        uint32_t j = 0, n_v = 0;  // tiles so far (their scores are in buffer j & 1), value tiles handed to the planning warp
+        bool ok = true;
+        const uint64_t qd = umma_desc_sw128(q_s);
+        auto release = [&](uint64_t* bar) {
+            if (lane == 0) umma_commit(smem_u32(bar));
+        };
+        auto scores = [&](uint32_t jj) {
+            for (int h = 0; h < Sh::HALVES; ++h, ++it) {
+                const int sl = it % Sh::SLOTS;
+                if (!wait(&hdr->full[sl], it / Sh::SLOTS, DEV_TIMEOUT_FULL)) return false;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t kd = umma_desc_sw128(ring + (uint32_t)sl * Sh::TILE_BYTES), qh = qd + (uint64_t)(h * (Sh::TILE_BYTES >> 4));
+#pragma unroll
+                    for (int k16 = 0; k16 < 8; ++k16) {
+                        const uint64_t off = (uint64_t)((k16 >> 2) * (AT_TILE * 128 >> 4) + (k16 & 3) * 2);
+                        umma_bf16(tmem + AT_COL_S + 128u * (jj & 1), qh + off, kd + off, Sh::IDESC_S(BF16), h > 0 || k16 > 0);
+                    }
+                }
+                release(&hdr->empty[sl]);
+            }
+            release(&hdr->s_full[jj & 1]);
+            return true;
+        };
+        for (int n = 0; ok && have_seg(n); done_seg(n), ++n) {
+            const AtSeg& w = hdr->seg[n % AT_SEGS];
+            const int t0 = w.t0, t1 = w.t1, d0 = w.d0, d1 = w.d1;
+            if (t0 >= t1) continue;
+            if (!wait(&hdr->q_full, q_no, DEV_TIMEOUT_FULL)) break;
+            ++q_no;
+            ok = scores(j) && (t0 + 1 >= t1 || scores(j + 1));
+            if (ok && t0 + 2 >= t1) release(&hdr->q_empty);
+            for (int t = t0; t < t1 && ok; ++t, ++j) {
+                const int s0 = it % Sh::SLOTS, s1 = (it + 1) % Sh::SLOTS;
+                ok = wait(&hdr->full[s0], it / Sh::SLOTS, DEV_TIMEOUT_FULL) && wait(&hdr->full[s1], (it + 1) / Sh::SLOTS, DEV_TIMEOUT_FULL);
+                if (ok && (t < d0 || t >= d1)) {  // rows that were not loaded are cleared by the planning warp
+                    if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ask));
+                    ok = wait(&hdr->v_ok, n_v++, DEV_TIMEOUT_FULL);
+                }
+                for (int part = 1; part >= 0 && ok; --part) {  // the second half of the keys first, as its probabilities come
+                    ok = wait(part ? &hdr->p_part[0] : &hdr->p_full[0], j, DEV_TIMEOUT_MMA);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        for (int h = 0; h < 2; ++h) {
+                            const uint64_t vd = umma_desc_v(ring + (uint32_t)(h ? s1 : s0) * Sh::TILE_BYTES);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                umma_ts(tmem + AT_COL_O + 128u * h, tmem + AT_COL_S + 128u * (j & 1) + AT_COL_P + 8u * (4 * part + k), vd + (uint64_t)((4 * part + k) * (2048 >> 4)),
+                                        Sh::IDESC_O(BF16), t > t0 || part == 0 || k > 0);
+                        }
+                    }
+                }
+                if (!ok) break;
+                release(&hdr->o_full[0]);
+                release(&hdr->empty[s0]);
+                release(&hdr->empty[s1]);
+                it += 2;
+                if (t + 2 < t1) {
+                    ok = scores(j + 2);
+                    if (t + 3 >= t1) release(&hdr->q_empty);
+                }
+            }
+        }
+        __syncwarp();
+        if (*cta_abort) {  // what was issued retires before the tensor memory is freed
+            if (lane == 0) {
+                umma_commit(smem_u32(&hdr->drain[0]));
+                const long long c0 = clock64();
+                while (!mbar_try_wait(smem_u32(&hdr->drain[0]), 0))
+                    if (clock64() - c0 > WAIT_LIMIT_CYCLES) {
+                        raise_status(DEV_TIMEOUT_DRAIN);
+                        break;
+                    }
+            }
+            __syncwarp();
+        }
+    } else if (!Sh::WIDE && (warp == Sh::MMA0 || warp == Sh::MMA1)) {
         // ------------------------------------------------------------ tensor cores: row tile i (one thread issues)
         // Both issuers follow every segment and every slot, also where there is no second row tile: a barrier whose phases one of
         // them skipped could not be waited for by parity.
-        const int i = warp == AT_WARP_MMA0 ? 0 : 1;
+        const int i = warp == Sh::MMA0 ? 0 : 1;
         const uint32_t d_s = tmem + AT_COL_S + 128u * i, d_o = tmem + AT_COL_O + 128u * i;
         const uint64_t qd = umma_desc_sw128(q_s + (uint32_t)i * Sh::TILE_BYTES);
         int it = 0, q_no = 0;
@@ -595,7 +689,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
         // ------------------------------------------------------------ softmax and epilogue: 16 rows per warp
         const int wg = warp >> 3, row0 = (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + (lane >> 2);  // this lane's rows: row0, row0 + 8
         const uint32_t lanes = (uint32_t)((warp & 3) * 32 + ((warp >> 2) & 1) * 16) << 16;
-        const uint32_t ts = tmem + lanes + AT_COL_S + 128u * wg, to = tmem + lanes + AT_COL_O + 128u * wg;
+        uint32_t ts = tmem + lanes + AT_COL_S + 128u * wg;
+        const uint32_t to = tmem + lanes + AT_COL_O + 128u * wg;
         uint32_t n_s = 0, n_o = 0, n_turn = 0;
         const float c = p.scale_log2;
         bool ok = true;
@@ -603,7 +698,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
             const AtSeg& w = hdr->seg[n % AT_SEGS];
             const int t0 = w.t0, t1 = w.t1, u0 = w.u0, u1 = w.u1, pos0 = w.kv - w.q_len;
             const int n_tok = w.tok1 - w.tok0;
-            const bool both = n_tok > tpt;
+            const bool both = !Sh::WIDE && n_tok > tpt;
             if (wg == 1 && !both) continue;  // no rows in this row tile
             int lo[2], hi[2];
 #pragma unroll
@@ -615,7 +710,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
             float m[2] = {-INFINITY, -INFINITY};
             uint64_t l2[2] = {0ull, 0ull};  // sums of this lane's even and odd columns
             for (int t = t0; t < t1; ++t) {
-                if (!wait(&hdr->s_full[wg], n_s, DEV_TIMEOUT_MMA)) {
+                if (Sh::WIDE) ts = tmem + lanes + AT_COL_S + 128u * (n_s & 1);
+                if (!wait(Sh::WIDE ? &hdr->s_full[n_s & 1] : &hdr->s_full[wg], Sh::WIDE ? n_s >> 1 : n_s, DEV_TIMEOUT_MMA)) {
                     ok = false;
                     break;
                 }
@@ -640,9 +736,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                     mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 2));
                     grew |= (mt[e] - m[e]) * c > 8.f || (m[e] == -INFINITY && mt[e] > -INFINITY);
                 }
+                bool o_done = !Sh::WIDE || t == t0;  // the outputs so far are complete (two row tiles: they are when the scores are)
                 if (t == t0) {
                     m[0] = mt[0], m[1] = mt[1];
                 } else if (__any_sync(0xffffffffu, grew)) {
+                    if (!o_done) {
+                        if (!wait(&hdr->o_full[0], n_o, DEV_TIMEOUT_MMA)) {
+                            ok = false;
+                            break;
+                        }
+                        ++n_o, o_done = true;
+                        tc_fence_after();
+                    }
                     float f[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -678,11 +783,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
                         if (left) mask_left(sr, t * AT_TILE, lo);
                     }
                     exp64<T>(sr, c, mc, ts + AT_COL_P + 32 * h, l2);
+                    if (h == 1 && !o_done) {  // once per tile, and before P is announced: the issuer is then past the P before
+                        ok = wait(&hdr->o_full[0], n_o, DEV_TIMEOUT_MMA);
+                        ++n_o;
+                    }
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(h ? &hdr->p_part[wg] : &hdr->p_full[wg]));  // the product of this half can begin
                 }
+                if (!ok) break;
                 if (both && lane == 0) mbar_arrive(smem_u32(&hdr->turn[wg ^ 1][warp & 3]));
             }
             if (!ok) break;
@@ -693,8 +803,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
             }
             const bool whole = w.begins && w.ends;
             const int slot = 2 * (int)blockIdx.x + (w.begins ? 1 : 0);
-            float* ml = whole ? nullptr : ArScratch<HD, AT_MAX_ROWS>::ml(p.scratch, gridDim.x, slot);
-            float* so = whole ? nullptr : ArScratch<HD, AT_MAX_ROWS>::o(p.scratch, gridDim.x, slot);
+            float* ml = whole ? nullptr : ArScratch<HD, Sh::MAX_ROWS>::ml(p.scratch, gridDim.x, slot);
+            float* so = whole ? nullptr : ArScratch<HD, Sh::MAX_ROWS>::o(p.scratch, gridDim.x, slot);
             {
                 // each lane its own columns, 8 or 4 bytes a time (turning them within the four lanes of a row for wider stores took
                 // three times the instructions, which are what bounds this part)
@@ -769,7 +879,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attn_tiles_kernel(const __grid_
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == AT_WARP_MMA0) {
+    if (warp == Sh::MMA0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -790,19 +900,21 @@ static int attn_tiles_inst(const AttnParams& p, const CUtensorMap& qm, const CUt
             if (dev >= 0 && dev < 64) configured[dev] = true;
         }
     }
-    const int tb = 2 * (AT_TILE / p.group), ctas = sm_count();
+    const int tb = AtShape<HD>::ROW_TILES * (AT_TILE / p.group), ctas = sm_count();
     const long items = ((long)p.total_q / tb + p.n_seqs) * p.nkv;  // at least as many as there are
     if (items > 1l << 30) return QMM_ERR_UNSUPPORTED;
     const int grid = p.stream_k ? ctas : (int)(items < ctas ? items : ctas);
-    if (int st = launch_overlapped(attn_tiles_kernel<T, HD>, dim3(grid), dim3(AT_THREADS), smem, s, qm, km, vm, p)) return st;
-    if (p.stream_k) return launch_overlapped(attn_join_kernel<HD, AT_MAX_ROWS>, dim3(ctas, AT_MAX_ROWS / 4), dim3(128), 0, s, p, ctas);
+    if (int st = launch_overlapped(attn_tiles_kernel<T, HD>, dim3(grid), dim3(AtShape<HD>::THREADS), smem, s, qm, km, vm, p)) return st;
+    if (p.stream_k) return launch_overlapped(attn_join_kernel<HD, AtShape<HD>::MAX_ROWS>, dim3(ctas, AtShape<HD>::MAX_ROWS / 4), dim3(128), 0, s, p, ctas);
     return QMM_OK;
 }
-static bool attn_tiles_fits(int hd) { return hd == 64 || hd == 96 || hd == 128; }
+static bool attn_tiles_fits(int hd) { return hd == 64 || hd == 96 || hd == 128 || hd == 256; }
+template <int HD> static long at_scratch_bytes_of() { return 4 * (long)ArScratch<HD, AtShape<HD>::MAX_ROWS>::floats(sm_count()); }
 static long attn_tiles_scratch_bytes(int hd) {
-    return 4 * (long)(hd == 64 ? ArScratch<64, AT_MAX_ROWS>::floats(sm_count()) : hd == 96 ? ArScratch<96, AT_MAX_ROWS>::floats(sm_count()) : ArScratch<128, AT_MAX_ROWS>::floats(sm_count()));
+    return hd == 64 ? at_scratch_bytes_of<64>() : hd == 96 ? at_scratch_bytes_of<96>() : hd == 128 ? at_scratch_bytes_of<128>() : at_scratch_bytes_of<256>();
 }
 // The queries as (element, head, row), a box = the rows of one row tile: tokens outermost, the heads of a group inside
+static int attn_tiles_rows(int hd) { return hd <= 128 ? 256 : 128; }  // of an item
 static int attn_tiles_launch(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, int dtype, int hd, cudaStream_t s) {
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return cuda_fail(cudaErrorNotSupported);
@@ -817,7 +929,8 @@ static int attn_tiles_launch(const AttnParams& p, const CUtensorMap& km, const C
     const bool f16 = dtype == QMM_DT_F16;
     if (hd == 64) return f16 ? attn_tiles_inst<__half, 64>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 64>(p, qm, km, vm, s);
     if (hd == 96) return f16 ? attn_tiles_inst<__half, 96>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 96>(p, qm, km, vm, s);
-    return f16 ? attn_tiles_inst<__half, 128>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 128>(p, qm, km, vm, s);
+    if (hd == 128) return f16 ? attn_tiles_inst<__half, 128>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 128>(p, qm, km, vm, s);
+    return f16 ? attn_tiles_inst<__half, 256>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 256>(p, qm, km, vm, s);
 }
 
 }  // namespace qmm
