@@ -64,14 +64,11 @@ static int check_out(const void* out, int dtype, long stride, int nqh, int hd) {
 }
 static bool bad_scale(float s) { return !(s > 0.f) || std::isinf(s); }
 
-// The three forms: up to 16 (token, query head of the group) rows per sequence and kv head (decode: bound by the cache), more
-// rows on tcgen05, more rows on mma.sync for the head dimensions that the tcgen05 kernel does not have.
-enum AttnForm { ATTN_NARROW, ATTN_TILES, ATTN_WIDE };
-static AttnForm attn_form(long max_q, int group, int hd) {
-    return max_q * group <= 16 ? ATTN_NARROW : attn_tiles_fits(hd) ? ATTN_TILES : ATTN_WIDE;
-}
-static int attn_run_form(AttnForm form, AttnParams& p, int dtype, int hd, long rows, long n_pages, cudaStream_t s) {
-    const int tile = form == ATTN_TILES ? AT_TILE : AR_TILE;
+// Up to 16 (token, query head of the group) rows per sequence and kv head: decode, bound by the cache (attn_rows.cu); more rows:
+// the tcgen05 form (attn_tiles.cu), whose tiles of 128 rows would be mostly empty below that
+static bool attn_narrow(long max_q, int group) { return max_q * group <= AR_ROWS; }
+static int attn_run(bool narrow, AttnParams& p, int dtype, int hd, long rows, long n_pages, cudaStream_t s) {
+    const int tile = narrow ? AR_TILE : AT_TILE;
     const int box = p.table ? gcd_int(p.page_size, tile) : tile;  // pages are multiples of 8, tiles powers of two
     for (p.box_shift = 3; 1 << p.box_shift < box;) ++p.box_shift;
     p.group_inv = (65536 + p.group - 1) / p.group;
@@ -79,8 +76,7 @@ static int attn_run_form(AttnForm form, AttnParams& p, int dtype, int hd, long r
     CUtensorMap km, vm;
     if (int st = kv_tensor_map(&km, p.k, dtype, hd, p.nkv, rows, n_pages, p.k_row, p.k_page, box)) return st;
     if (int st = kv_tensor_map(&vm, p.v, dtype, hd, p.nkv, rows, n_pages, p.v_row, p.v_page, box)) return st;
-    if (form == ATTN_TILES) return attn_tiles_launch(p, km, vm, dtype, hd, s);
-    return attn_rows_launch(p, km, vm, dtype, hd, form == ATTN_NARROW, s);
+    return narrow ? attn_rows_launch(p, km, vm, dtype, hd, s) : attn_tiles_launch(p, km, vm, dtype, hd, s);
 }
 
 }  // namespace qmm
@@ -132,8 +128,7 @@ int launch_rope_kv_append_paged(const void* qkv, int qkv_dtype, long qkv_stride,
 long qmm_attn_paged_scratch_bytes(int max_q, int n_q_heads, int n_kv_heads, int head_dim) {
     if (max_q < 0) return QMM_ERR_SHAPE;
     if (int st = check_heads(n_q_heads, n_kv_heads, head_dim)) return st;
-    const AttnForm form = attn_form(max_q, n_q_heads / n_kv_heads, head_dim);
-    return form == ATTN_TILES ? attn_tiles_scratch_bytes(head_dim) : attn_rows_scratch_bytes(head_dim, form == ATTN_NARROW);
+    return attn_narrow(max_q, n_q_heads / n_kv_heads) ? attn_rows_scratch_bytes(head_dim) : attn_tiles_scratch_bytes(head_dim);
 }
 
 int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, const qmm_seq_batch* seqs, void* out, int out_dtype, long out_stride,
@@ -157,11 +152,10 @@ int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, cons
     p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = seqs->max_kv;
     p.nqh = n_q_heads, p.nkv = nkv, p.group = n_q_heads / nkv, p.window = window, p.out_dtype = out_dtype;
     p.scale_log2 = kq_scale * 1.4426950408889634f;
-    // decode, and more rows where their items would not fill the GPU several times over: the tiles are shared evenly
-    const AttnForm form = attn_form(seqs->max_q, p.group, hd);
-    const long items = ((long)p.total_q * p.group / (form == ATTN_TILES ? attn_tiles_rows(hd) : 64) + 1) * nkv;
-    p.stream_k = form == ATTN_NARROW || items < 4l * sm_count();
-    return attn_run_form(form, p, kv->dtype, hd, p.page_size, p.n_pages, as_stream(stream));
+    // more rows whose items would not fill the GPU several times over: their tiles are shared evenly, as those of decode always are
+    const bool narrow = attn_narrow(seqs->max_q, p.group);
+    p.stream_k = ((long)p.total_q * p.group / attn_tiles_rows(hd) + 1) * nkv < 4l * sm_count();
+    return attn_run(narrow, p, kv->dtype, hd, p.page_size, p.n_pages, as_stream(stream));
 }
 
 int launch_attn_packed(const void* q, const void* k, const void* v, int dtype, long q_stride, long k_stride, long v_stride,
@@ -186,7 +180,7 @@ int launch_attn_packed(const void* q, const void* k, const void* v, int dtype, l
     p.nqh = n_q_heads, p.nkv = nkv, p.group = n_q_heads / nkv, p.window = window, p.out_dtype = out_dtype;
     p.scale_log2 = kq_scale * 1.4426950408889634f;
     p.k_page = (long)p.total_q * k_stride, p.v_page = (long)p.total_q * v_stride;  // one page of all rows
-    return attn_run_form(attn_tiles_fits(hd) ? ATTN_TILES : ATTN_WIDE, p, dtype, hd, p.total_q, 1, as_stream(stream));
+    return attn_run(false, p, dtype, hd, p.total_q, 1, as_stream(stream));
 }
 
 }  // extern "C"

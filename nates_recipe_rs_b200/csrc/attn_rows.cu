@@ -1,14 +1,12 @@
-// Attention of new tokens over a paged cache (or over packed prompts) on mma.sync: any head dimension of the library, any
-// number of rows.  The counterpart, for a batch of sequences of different lengths, of the upstream's gpu_gqa_attn_into
+// Attention of one or a few new tokens per sequence over a paged cache (decode) on mma.sync.  The counterpart, for a batch of sequences of different lengths, of the upstream's gpu_gqa_attn_into
 // (gpu-core/src/infer_ops.rs:160-189).
 //
 //   out[r, h] = sum_t w_t V_t / sum_t w_t,  w_t = exp(kq_scale * q_r . K_t - max),  t in (pos_r - window, pos_r]
 //
-// One pass over the keys with a running maximum and sum.  The rows of a work item are (token, query head of the group) pairs
-// of ONE kv head, so a tile of keys and values fetched once serves every query head that shares it.  Decode (WM = 1, up to 16
-// rows: bound by the cache bytes): the four math warps take 16 keys each of a tile of 64 and join at the end; a fifth warp
-// keeps TMA copies of the next tiles in flight.  More rows (WM = 4, 64 rows: bound by mma.sync): a warp takes 16 rows and all
-// the keys of a tile.
+// One pass over the keys with a running maximum and sum.  The rows of a work item (up to 16) are (token, query head of the group)
+// pairs of ONE kv head, so a tile of keys and values fetched once serves every query head that shares it.  Bound by the cache bytes:
+// the four math warps take 16 keys each of a tile of 64 and join at the end; a fifth warp plans and keeps TMA copies of the next
+// tiles in flight.
 // Few items over a long axis: all (item, tile) pairs are shared out evenly over the CTAs, whatever the sequences' lengths
 // (read on the device: nothing is copied to the host).  A CTA's share begins and ends inside at most two items; those go to
 // scratch as (maximum, sum, unnormalised output) and attn_join_kernel adds them in key order, so reruns are bit identical.
@@ -19,12 +17,13 @@
 namespace qmm {
 
 constexpr int AR_TILE = 64;       // keys per tile
+constexpr int AR_ROWS = 16;       // rows of an item
 constexpr int AR_THREADS = 160;   // four math warps and the copying warp
-template <int HD, int WM> struct ArShape {
+template <int HD> struct ArShape {
     static constexpr int NCH = (HD + 63) / 64;
     static constexpr int TILE_BYTES = NCH * AR_TILE * 128;  // one matrix
-    // two CTAs per SM up to 128 elements: about 96 KB (decode: bytes in flight) or 64 KB (many rows) of tiles each
-    static constexpr int STAGES = WM == 1 ? (HD <= 64 ? 6 : 3) : (HD <= 64 ? 4 : 2);
+    // two CTAs per SM up to 128 elements, about 96 KB of tiles each (bytes in flight); one with 192 KB at 256
+    static constexpr int STAGES = HD <= 64 ? 6 : 3;
     static constexpr int CTAS_PER_SM = HD <= 128 ? 2 : 1;
     static constexpr int BUF_PITCH = HD + 4;
     static constexpr bool Q_REGS = HD <= 128;  // the queries stay in registers (wider heads read them from shared memory)
@@ -54,10 +53,9 @@ struct __align__(16) ArHeader {
     int abort_flag;
 };
 
-template <int HD, int WM> constexpr size_t ar_smem_bytes() {
-    using Sh = ArShape<HD, WM>;
-    return 1024 + (size_t)Sh::STAGES * 2 * Sh::TILE_BYTES + (size_t)16 * WM * (Sh::NCH * 64 + 8) * 2 + (WM == 1 ? 16 * Sh::BUF_PITCH * 4 : 0) +
-           sizeof(ArHeader);
+template <int HD> constexpr size_t ar_smem_bytes() {
+    using Sh = ArShape<HD>;
+    return 1024 + (size_t)Sh::STAGES * 2 * Sh::TILE_BYTES + (size_t)AR_ROWS * (Sh::NCH * 64 + 8) * 2 + AR_ROWS * Sh::BUF_PITCH * 4 + sizeof(ArHeader);
 }
 
 // What a CTA leaves in scratch for attn_join_kernel: the item that begins in it and continues in later CTAs
@@ -95,11 +93,10 @@ __device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 128;" ::
 __device__ __forceinline__ int ar_tile_count(const KeyRange& kr) { return max(1, (max(kr.b, 0) + AR_TILE - 1) / AR_TILE - kr.a / AR_TILE); }
 constexpr int AR_ITEM_COST = 2;
 
-// Walks the segments (item, tiles of it) of this CTA (the copying warp).  An item is (sequence, kv head, block of R rows); all items
+// Walks the segments (item, tiles of it) of this CTA (the copying warp).  An item is (sequence, kv head, block of AR_ROWS rows); all items
 // of a sequence count the tiles of the whole sequence, at least one, and AR_ITEM_COST more for what an item costs beside its tiles
 // (its queries, the joining of its warps, its outputs): without that the CTAs that got the short sequences finished last.  A share
 // that begins or ends among those extra places begins or ends where the item does.
-template <int R>
 struct ArWalker {
     const AttnParams& p;
     long left;         // places of this CTA's share still to come
@@ -112,7 +109,7 @@ struct ArWalker {
         const KeyRange kr = key_range(p, si, 0, si.q_len);
         tl = kr.a / AR_TILE;
         nt = ar_tile_count(kr);
-        nrb = (si.q_len * p.group + R - 1) / R;
+        nrb = (si.q_len * p.group + AR_ROWS - 1) / AR_ROWS;
     }
     __device__ __forceinline__ bool next(ArSeg& g) {
         if (left <= 0) return false;
@@ -130,22 +127,19 @@ struct ArWalker {
         left -= n, within = w1;
         g.more = nt + AR_ITEM_COST - w1;
         if (g.ends) within = 0, ++item;
-        g.r0 = rb * R, g.n_rows = min(R, si.q_len * p.group - g.r0);
+        g.r0 = rb * AR_ROWS, g.n_rows = min(AR_ROWS, si.q_len * p.group - g.r0);
         const KeyRange kr = key_range(p, si, g.r0 / p.group, (g.r0 + g.n_rows - 1) / p.group + 1);
         g.t0 = max(g.st0, kr.a / AR_TILE), g.t1 = min(g.st1, (kr.b + AR_TILE - 1) / AR_TILE);
         g.a2 = kr.a2, g.b2 = kr.b2, g.c0 = (kr.a >> p.box_shift) << p.box_shift;
         return true;
     }
 };
-template <int R> struct ArTiles {  // tiles of all items of a sequence
+struct ArTiles {  // tiles of all items of a sequence
     __device__ static __forceinline__ long count(const AttnParams& p, int s) {
         const SeqInfo si = seq_info(p, s);
         const KeyRange kr = key_range(p, si, 0, si.q_len);
-        return (long)((si.q_len * p.group + R - 1) / R) * p.nkv * (ar_tile_count(kr) + AR_ITEM_COST);
+        return (long)((si.q_len * p.group + AR_ROWS - 1) / AR_ROWS) * p.nkv * (ar_tile_count(kr) + AR_ITEM_COST);
     }
-};
-template <int R> struct ArBlocks {  // row blocks of a sequence
-    __device__ static __forceinline__ long count(const AttnParams& p, int s) { return (seq_info(p, s).q_len * p.group + R - 1) / R; }
 };
 // First tile of CTA c of n when `total` tiles are shared evenly
 __device__ __noinline__ long ar_share(long total, int c, int n) { return total * c / n; }
@@ -183,18 +177,18 @@ template <int HD, int R> struct ArScratch {  // layout of the scratch: joins, th
     __device__ static float* o(float* base, int ctas, int slot) { return base + join_floats(ctas) + (size_t)ctas * 2 * R * 2 + (size_t)slot * R * HD; }
 };
 
-template <typename T, int HD, int WM>
-__global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) attn_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+template <typename T, int HD>
+__global__ void __launch_bounds__(AR_THREADS, ArShape<HD>::CTAS_PER_SM) attn_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                                                const __grid_constant__ AttnParams params) {
-    using Sh = ArShape<HD, WM>;
-    constexpr int R = 16 * WM, WN = 4 / WM, KW = AR_TILE / WN;  // rows of an item, warps along the keys, keys per warp and tile
-    constexpr int NT = KW / 8, QPITCH = Sh::NCH * 64 + 8;
+    using Sh = ArShape<HD>;
+    using Scratch = ArScratch<HD, AR_ROWS>;
+    constexpr int KW = AR_TILE / 4, NT = KW / 8, QPITCH = Sh::NCH * 64 + 8;
     extern __shared__ __align__(1024) uint8_t ar_raw[];
     uint8_t* sm = ar_raw + ((1024u - (smem_u32(ar_raw) & 1023u)) & 1023u);
     const uint32_t ring = smem_u32(sm);
     T* qs = reinterpret_cast<T*>(sm + (size_t)Sh::STAGES * 2 * Sh::TILE_BYTES);
-    float* buf = reinterpret_cast<float*>(qs + R * QPITCH);  // (WM == 1) one 16 x HD output while the warps join
-    ArHeader* hdr = reinterpret_cast<ArHeader*>(reinterpret_cast<uint8_t*>(buf) + (WM == 1 ? 16 * Sh::BUF_PITCH * 4 : 0));
+    float* buf = reinterpret_cast<float*>(qs + AR_ROWS * QPITCH);  // one 16 x HD output while the warps join
+    ArHeader* hdr = reinterpret_cast<ArHeader*>(reinterpret_cast<uint8_t*>(buf) + AR_ROWS * Sh::BUF_PITCH * 4);
     const AttnParams& p = hdr->p;
     volatile int* cta_abort = &hdr->abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -215,39 +209,27 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
     int n_ctas = 1, first_seq = 0;
     long total = 0, before = 0, share = 0;  // places of the whole batch, before the sequence and before this CTA's share
     if (p.n_seqs > AR_FEW_SEQS) {
-        if (p.stream_k) {
-            find_item<ArTiles<R>>(p, 1l << 62, total, hdr->scan);
-            n_ctas = ar_ctas(total, gridDim.x);
-            share = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
-            first_seq = find_item<ArTiles<R>>(p, share, before, hdr->scan);
-        } else {
-            first_seq = find_item<ArBlocks<R>>(p, blockIdx.y, before, hdr->scan);
-        }
+        find_item<ArTiles>(p, 1l << 62, total, hdr->scan);
+        n_ctas = ar_ctas(total, gridDim.x);
+        share = ar_share(total, min((int)blockIdx.x, n_ctas), n_ctas);
+        first_seq = find_item<ArTiles>(p, share, before, hdr->scan);
     }
     int it = 0;  // tiles so far, over all segments: stage it % STAGES
 
     if (warp == 4) {
         // ------------------------------------------------------------ plan and copies
-        ArWalker<R> w{p};
-        if (p.n_seqs <= AR_FEW_SEQS) {
-            if (p.stream_k) first_seq = plan_few<ArTiles<R>>(p, total, n_ctas, share, before);
-            else first_seq = warp_find_item<ArBlocks<R>>(p, blockIdx.y, before);
-        }
+        ArWalker w{p};
+        if (p.n_seqs <= AR_FEW_SEQS) first_seq = plan_few<ArTiles>(p, total, n_ctas, share, before);
         w.left = 0, w.s = first_seq, w.item = w.within = w.nrb = 0;
-        if (p.stream_k && lane == 0) {
+        if (lane == 0) {
             (reinterpret_cast<ArJoin*>(p.scratch) + blockIdx.x)->n_rows = 0;
             hdr->scan[34] = total, hdr->scan[35] = n_ctas;
         }
-        if (first_seq >= 0 && (!p.stream_k || (int)blockIdx.x < n_ctas)) {  // else: nothing for this CTA
+        if (first_seq >= 0 && (int)blockIdx.x < n_ctas) {  // else: nothing for this CTA
             w.load_seq();
-            if (p.stream_k) {
-                w.left = ar_share(total, blockIdx.x + 1, n_ctas) - share;
-                const long ahead = share - before;
-                w.item = (int)(ahead / (w.nt + AR_ITEM_COST)), w.within = (int)(ahead - (long)w.item * (w.nt + AR_ITEM_COST));
-            } else {  // one item per CTA: row block blockIdx.y of all (a sequence's last, longest, first), kv head blockIdx.x
-                w.left = w.nt + AR_ITEM_COST, w.within = 0;
-                w.item = blockIdx.x * w.nrb + (w.nrb - 1 - (int)(blockIdx.y - before));
-            }
+            w.left = ar_share(total, blockIdx.x + 1, n_ctas) - share;
+            const long ahead = share - before;
+            w.item = (int)(ahead / (w.nt + AR_ITEM_COST)), w.within = (int)(ahead - (long)w.item * (w.nt + AR_ITEM_COST));
         }
         int q_no = 0;
         for (int n = 0; !*cta_abort; ++n) {
@@ -308,7 +290,7 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
 
     // ---------------------------------------------------------------- math warps
     const int qr = lane >> 2, pq = lane & 3;
-    const int row_w = WM == 1 ? 0 : 16 * warp, key_w = WM == 1 ? KW * warp : 0;  // this warp's rows and keys of a tile
+    const int key_w = KW * warp;  // this warp's keys of a tile
     for (int sn = 0;; ++sn) {
         // (a wait that runs out does not end a math warp's run over the segments it knows of: the warps meet at barriers; without
         // a next segment all four stop alike)
@@ -322,13 +304,13 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
         int lo[2], hi[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int r = row_w + qr + 8 * e;
+            const int r = qr + 8 * e;
             const int pos = pos0 + (r0 + r) / p.group;
             hi[e] = r < n_rows ? max(pos + 1, 0) : 0;
             lo[e] = p.window ? max(0, pos - p.window + 1) : 0;
         }
         uint32_t qf[Sh::Q_REGS ? HD / 16 : 1][4];
-        const uint32_t qa = smem_u32(qs + (row_w + (lane & 15)) * QPITCH + (lane >> 4) * 8);
+        const uint32_t qa = smem_u32(qs + (lane & 15) * QPITCH + (lane >> 4) * 8);
         if constexpr (Sh::Q_REGS) {
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk) ldsm_x4(qf[kk], qa + kk * 32);
@@ -444,8 +426,8 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
         // where the segment's result goes: the output rows, or a slot of scratch (0: continues an item, 1: begins one)
         const bool whole = w.begins && w.ends;
         const int slot = 2 * (int)blockIdx.x + (w.begins ? 1 : 0);
-        float* sml = whole ? nullptr : ArScratch<HD, R>::ml(p.scratch, gridDim.x, slot);
-        float* so = whole ? nullptr : ArScratch<HD, R>::o(p.scratch, gridDim.x, slot);
+        float* sml = whole ? nullptr : Scratch::ml(p.scratch, gridDim.x, slot);
+        float* so = whole ? nullptr : Scratch::o(p.scratch, gridDim.x, slot);
         auto out_elem = [&](int r) {  // element index of row r's first output
             const int tok = (r0 + r) / p.group, h = w.kvh * p.group + (r0 + r) % p.group;
             return (size_t)(w.q0 + tok) * p.out_stride + (size_t)h * HD;
@@ -457,7 +439,7 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
         float odd[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) odd[0] += (o[i][0] + o[i][1]) * 0.f, odd[1] += (o[i][2] + o[i][3]) * 0.f;
-        if (bar_any((odd[0] != odd[0] && row_w + qr < n_rows) || (odd[1] != odd[1] && row_w + qr + 8 < n_rows))) {
+        if (bar_any((odd[0] != odd[0] && qr < n_rows) || (odd[1] != odd[1] && qr + 8 < n_rows))) {
 #pragma unroll 1
             for (int r = warp; r < n_rows; r += 4) {
                 const int tok = (r0 + r) / p.group, pos = pos0 + tok;
@@ -472,7 +454,7 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
                 }
                 if (!whole && lane == 0) sml[2 * r] = em, sml[2 * r + 1] = el;
             }
-        } else if constexpr (WM == 1) {
+        } else {
             // the four warps' parts, added through one buffer in a fixed order
             if (pq == 0)
 #pragma unroll
@@ -517,22 +499,6 @@ __global__ void __launch_bounds__(AR_THREADS, (ArShape<HD, WM>::CTAS_PER_SM)) at
                 } else {
                     *reinterpret_cast<float2*>(so + (size_t)r * HD + c) = x;
                     if (c == 0) sml[2 * r] = mm, sml[2 * r + 1] = ll;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = row_w + qr + 8 * e;
-                if (r < n_rows) {
-                    const bool sees = row_sees(r);
-                    const float inv = sees ? 1.f / l[e] : 0.f;
-                    const size_t oe = out_elem(r);
-#pragma unroll
-                    for (int n = 0; n < HD / 8; ++n) {
-                        if (whole) store_out2(p.out, p.out_dtype, oe + 8 * n + 2 * pq, sees ? o[n][2 * e] * inv : 0.f, sees ? o[n][2 * e + 1] * inv : 0.f);
-                        else *reinterpret_cast<float2*>(so + (size_t)r * HD + 8 * n + 2 * pq) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
-                    }
-                    if (!whole && pq == 0) sml[2 * r] = m[e], sml[2 * r + 1] = l[e];
                 }
             }
         }
@@ -626,10 +592,9 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
 }
 
 // ---- host side ----
-template <typename T, int HD, int WM>
+template <typename T, int HD>
 static int attn_rows_inst(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
-    constexpr int R = 16 * WM;
-    constexpr size_t smem = ar_smem_bytes<HD, WM>();
+    constexpr size_t smem = ar_smem_bytes<HD>();
     static std::mutex mu;
     static bool configured[64] = {};
     int dev = 0;
@@ -637,45 +602,36 @@ static int attn_rows_inst(const AttnParams& p, const CUtensorMap& km, const CUte
     {
         std::lock_guard<std::mutex> g(mu);
         if (dev < 0 || dev >= 64 || !configured[dev]) {
-            QMM_CUDA_TRY(cudaFuncSetAttribute(attn_rows_kernel<T, HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            QMM_CUDA_TRY(cudaFuncSetAttribute(attn_rows_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             if (dev >= 0 && dev < 64) configured[dev] = true;
         }
     }
-    const int ctas = sm_count() * ArShape<HD, WM>::CTAS_PER_SM;
-    const long blocks = (long)p.total_q * p.group / R + p.n_seqs;  // at least as many as row blocks there are
-    dim3 grid = p.stream_k ? dim3(ctas) : dim3(p.nkv, (unsigned)blocks);
-    if (!p.stream_k && blocks > 65535) return QMM_ERR_UNSUPPORTED;
-    if (int st = launch_overlapped(attn_rows_kernel<T, HD, WM>, grid, dim3(AR_THREADS), smem, s, km, vm, p)) return st;
-    if (p.stream_k) return launch_overlapped(attn_join_kernel<HD, R>, dim3(ctas, R / 4), dim3(128), 0, s, p, ctas);
-    return QMM_OK;
+    const int ctas = sm_count() * ArShape<HD>::CTAS_PER_SM;
+    if (int st = launch_overlapped(attn_rows_kernel<T, HD>, dim3(ctas), dim3(AR_THREADS), smem, s, km, vm, p)) return st;
+    return launch_overlapped(attn_join_kernel<HD, AR_ROWS>, dim3(ctas, AR_ROWS / 4), dim3(128), 0, s, p, ctas);
 }
 
-template <int HD, int WM> static long ar_scratch_bytes_of() { return 4 * (long)ArScratch<HD, 16 * WM>::floats(sm_count() * ArShape<HD, WM>::CTAS_PER_SM); }
-static long attn_rows_scratch_bytes(int hd, bool narrow) {
+template <int HD> static long ar_scratch_bytes_of() { return 4 * (long)ArScratch<HD, AR_ROWS>::floats(sm_count() * ArShape<HD>::CTAS_PER_SM); }
+static long attn_rows_scratch_bytes(int hd) {
     switch (hd) {
-    case 32: return narrow ? ar_scratch_bytes_of<32, 1>() : ar_scratch_bytes_of<32, 4>();
-    case 64: return ar_scratch_bytes_of<64, 1>();
-    case 96: return ar_scratch_bytes_of<96, 1>();
-    case 128: return ar_scratch_bytes_of<128, 1>();
-    case 256: return ar_scratch_bytes_of<256, 1>();
+    case 32: return ar_scratch_bytes_of<32>();
+    case 64: return ar_scratch_bytes_of<64>();
+    case 96: return ar_scratch_bytes_of<96>();
+    case 128: return ar_scratch_bytes_of<128>();
+    case 256: return ar_scratch_bytes_of<256>();
     }
     return QMM_ERR_UNSUPPORTED;
 }
 
-// narrow: up to 16 rows per item; otherwise (head_dim 32 only: the others have attn_tiles.cu) 64
-static int attn_rows_launch(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, int dtype, int hd, bool narrow, cudaStream_t s) {
+static int attn_rows_launch(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, int dtype, int hd, cudaStream_t s) {
     const bool f16 = dtype == QMM_DT_F16;
-#define QMM_AR_CASE(HD_, WM_) return f16 ? attn_rows_inst<__half, HD_, WM_>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, HD_, WM_>(p, km, vm, s)
     switch (hd) {
-    case 32:
-        if (narrow) QMM_AR_CASE(32, 1);
-        QMM_AR_CASE(32, 4);
-    case 64: QMM_AR_CASE(64, 1);
-    case 96: QMM_AR_CASE(96, 1);
-    case 128: QMM_AR_CASE(128, 1);
-    case 256: QMM_AR_CASE(256, 1);
+    case 32: return f16 ? attn_rows_inst<__half, 32>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, 32>(p, km, vm, s);
+    case 64: return f16 ? attn_rows_inst<__half, 64>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, 64>(p, km, vm, s);
+    case 96: return f16 ? attn_rows_inst<__half, 96>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, 96>(p, km, vm, s);
+    case 128: return f16 ? attn_rows_inst<__half, 128>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, 128>(p, km, vm, s);
+    case 256: return f16 ? attn_rows_inst<__half, 256>(p, km, vm, s) : attn_rows_inst<__nv_bfloat16, 256>(p, km, vm, s);
     }
-#undef QMM_AR_CASE
     return QMM_ERR_UNSUPPORTED;
 }
 

@@ -1,5 +1,5 @@
-// Attention of many rows over a paged cache or over packed prompts on tcgen05: pieces of prompts and whole prompts, head_dim 64,
-// 96 and 128.  Same operator and same conventions as attn_rows.cu.
+// Attention of many rows over a paged cache or over packed prompts on tcgen05: pieces of prompts and whole prompts.  Same
+// operator and same conventions as attn_rows.cu.
 //
 // A CTA owns up to two tiles of 128 rows of one kv head; a row is a (token, query head of the group) pair, tokens outermost, so
 // one tile of keys and values serves every query head that shares it and a tile spans few positions (128 / group tokens: little
@@ -908,10 +908,16 @@ static int attn_tiles_inst(const AttnParams& p, const CUtensorMap& qm, const CUt
     if (p.stream_k) return launch_overlapped(attn_join_kernel<HD, AtShape<HD>::MAX_ROWS>, dim3(ctas, AtShape<HD>::MAX_ROWS / 4), dim3(128), 0, s, p, ctas);
     return QMM_OK;
 }
-static bool attn_tiles_fits(int hd) { return hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 template <int HD> static long at_scratch_bytes_of() { return 4 * (long)ArScratch<HD, AtShape<HD>::MAX_ROWS>::floats(sm_count()); }
 static long attn_tiles_scratch_bytes(int hd) {
-    return hd == 64 ? at_scratch_bytes_of<64>() : hd == 96 ? at_scratch_bytes_of<96>() : hd == 128 ? at_scratch_bytes_of<128>() : at_scratch_bytes_of<256>();
+    switch (hd) {
+    case 32: return at_scratch_bytes_of<32>();
+    case 64: return at_scratch_bytes_of<64>();
+    case 96: return at_scratch_bytes_of<96>();
+    case 128: return at_scratch_bytes_of<128>();
+    case 256: return at_scratch_bytes_of<256>();
+    }
+    return QMM_ERR_UNSUPPORTED;
 }
 // The queries as (element, head, row), a box = the rows of one row tile: tokens outermost, the heads of a group inside
 static int attn_tiles_rows(int hd) { return hd <= 128 ? 256 : 128; }  // of an item
@@ -927,10 +933,14 @@ static int attn_tiles_launch(const AttnParams& p, const CUtensorMap& km, const C
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cuda_fail(cudaErrorInvalidValue);
     const bool f16 = dtype == QMM_DT_F16;
-    if (hd == 64) return f16 ? attn_tiles_inst<__half, 64>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 64>(p, qm, km, vm, s);
-    if (hd == 96) return f16 ? attn_tiles_inst<__half, 96>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 96>(p, qm, km, vm, s);
-    if (hd == 128) return f16 ? attn_tiles_inst<__half, 128>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 128>(p, qm, km, vm, s);
-    return f16 ? attn_tiles_inst<__half, 256>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 256>(p, qm, km, vm, s);
+    switch (hd) {
+    case 32: return f16 ? attn_tiles_inst<__half, 32>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 32>(p, qm, km, vm, s);
+    case 64: return f16 ? attn_tiles_inst<__half, 64>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 64>(p, qm, km, vm, s);
+    case 96: return f16 ? attn_tiles_inst<__half, 96>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 96>(p, qm, km, vm, s);
+    case 128: return f16 ? attn_tiles_inst<__half, 128>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 128>(p, qm, km, vm, s);
+    case 256: return f16 ? attn_tiles_inst<__half, 256>(p, qm, km, vm, s) : attn_tiles_inst<__nv_bfloat16, 256>(p, qm, km, vm, s);
+    }
+    return QMM_ERR_UNSUPPORTED;
 }
 
 }  // namespace qmm
