@@ -1,5 +1,5 @@
 // What the operators on a paged KV cache share: the view of a batch of sequences and of the cache, the tensor maps through
-// which tiles of keys and values arrive, and the exact (slow) attention of one row.
+// which tiles of keys and values arrive, and what is done about values that are not finite under a mask.
 //
 // A batch is packed: the new tokens of sequence s are rows cu_q[s] .. cu_q[s+1]-1; row i of them is position
 // kv_len[s] - q_len + i.  Position t of a sequence lies in page table[s][t / page_size], slot t % page_size.  A packed
@@ -206,11 +206,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(r), "r"(pg), "r"(bar)
                  : "memory");
 }
-// The boxes of tile `t` (TILE positions) that hold a key of [a, kv): first, and how many.  What no box covers, and what lies past
-// kv in the last one, is whatever was there before: the reader clears those rows (of the values; scores are masked).
+// The boxes of tile `t` (TILE positions) that hold a key of [a, b), the keys that some row sees: first, and how many.  What no box
+// covers is whatever was there before: the reader clears the rows outside [a, b) (of the values; scores are masked).
 template <int TILE>
-__device__ __forceinline__ void tile_boxes(const AttnParams& p, int t, int a, int kv, int& first, int& count) {
-    const int lo = max(a - t * TILE, 0), hi = min(kv - t * TILE, TILE);
+__device__ __forceinline__ void tile_boxes(const AttnParams& p, int t, int a, int b, int& first, int& count) {
+    const int lo = max(a - t * TILE, 0), hi = min(b - t * TILE, TILE);
     first = lo >> p.box_shift;
     count = hi > lo ? ((hi - 1) >> p.box_shift) - first + 1 : 0;
 }
@@ -237,43 +237,99 @@ __device__ __forceinline__ int page_of_boxes(const AttnParams& p, int s, int row
     return page_of(p, s, idx);
 }
 
-// ---- one row, exactly by the formula: keys [k0, k1) of those the row sees, one warp, lane l holds elements l + 32 j ----
-// The tensor cores add 0 * v for a masked key, which is not 0 when v is an infinity or a NaN: rows whose output is not finite are
-// computed again this way (where that is what the formula gives, it stays).  m is in units of the raw score.
-template <typename T, int HD>
-__device__ __noinline__ void attn_row_exact(const AttnParams& p, int s, int q0, int tok, int head, int kvh, int k0, int k1, float& m, float& l,
-                                            float (&o)[HD / 32]) {
-    const int lane = threadIdx.x & 31;
-    const T* qr = static_cast<const T*>(p.q) + (size_t)(q0 + tok) * p.q_stride + (size_t)head * HD;
-    float qv[HD / 32];
+// ---- values that are not finite under a mask ----
+// The tensor cores add 0 * v for a masked key, which is not 0 when v is an infinity or a NaN.  So in the keys that some rows of an
+// item see and others do not, such values are made zeros in shared memory (clean_value), and added to the outputs of the rows that
+// do see them afterwards (add_odd_values): v + anything is v or NaN, whatever its weight, so no product is needed.
+// Eight 16-bit values: those that are not finite become zeros; returns whether there were any
+template <typename T> __device__ __forceinline__ bool odd_word(uint32_t w);  // of two values
+template <> __device__ __forceinline__ bool odd_word<__half>(uint32_t w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }
+template <> __device__ __forceinline__ bool odd_word<__nv_bfloat16>(uint32_t w) { return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u; }
+template <typename T> __device__ __forceinline__ uint32_t clean_word(uint32_t w) {
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    if ((w & E) == E) w &= 0xFFFF0000u;
+    if ((w & (E << 16)) == E << 16) w &= 0x0000FFFFu;
+    return w;
+}
+template <typename T> __device__ __forceinline__ uint32_t times_zero(uint32_t w, uint32_t acc);  // acc + 0 * w: 0, or NaN
+template <> __device__ __forceinline__ uint32_t times_zero<__half>(uint32_t w, uint32_t acc) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&w), __half2(__half(0.f), __half(0.f)), *reinterpret_cast<const __half2*>(&acc));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <> __device__ __forceinline__ uint32_t times_zero<__nv_bfloat16>(uint32_t w, uint32_t acc) {
+    const __nv_bfloat162 z = __floats2bfloat162_rn(0.f, 0.f), r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w), z, *reinterpret_cast<const __nv_bfloat162*>(&acc));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Rows [r0, r1) of one chunk of a value tile (8 pieces of 16 bytes a row): those outside [z0, z1) become zeros, the others are
+// cleaned.  `threads` threads, this one number `i0`, U pieces in flight each.  Returns whether a value was made zero that some row
+// sees.
+template <typename T, int U>
+__device__ __forceinline__ bool clear_values(uint4* chunk, int r0, int r1, int z0, int z1, int i0, int threads) {
+    z0 = min(max(z0, r0), r1), z1 = min(max(z1, z0), r1);
+#pragma unroll 4
+    for (int i = r0 * 8 + i0; i < z0 * 8; i += threads) chunk[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 4
+    for (int i = z1 * 8 + i0; i < r1 * 8; i += threads) chunk[i] = make_uint4(0u, 0u, 0u, 0u);
+    bool odd = false;
+#pragma unroll 1
+    for (int b = z0 * 8 + i0; b < z1 * 8; b += U * threads) {
+        uint4 y[U];
 #pragma unroll
-    for (int j = 0; j < HD / 32; ++j) qv[j] = to_f32<T>(qr[lane + 32 * j]), o[j] = 0.f;
-    m = -INFINITY, l = 0.f;
+        for (int u = 0; u < U; ++u) y[u] = b + u * threads < z1 * 8 ? chunk[b + u * threads] : make_uint4(0u, 0u, 0u, 0u);
+        uint32_t a0 = 0u, a1 = 0u, a2 = 0u, a3 = 0u;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            a0 = times_zero<T>(y[u].x, a0), a1 = times_zero<T>(y[u].y, a1), a2 = times_zero<T>(y[u].z, a2), a3 = times_zero<T>(y[u].w, a3);
+        if (!(odd_word<T>(a0) || odd_word<T>(a1) || odd_word<T>(a2) || odd_word<T>(a3))) continue;
+        odd = true;
+#pragma unroll 1
+        for (int i = b; i < min(b + U * threads, z1 * 8); i += threads) {
+            uint4 x = chunk[i];
+            x.x = clean_word<T>(x.x), x.y = clean_word<T>(x.y), x.z = clean_word<T>(x.z), x.w = clean_word<T>(x.w);
+            chunk[i] = x;
+        }
+    }
+    return odd;
+}
+__device__ __forceinline__ float load_out1(const void* out, int dtype, size_t e) {
+    return dtype == QMM_DT_F32 ? static_cast<const float*>(out)[e] : dtype == QMM_DT_F16 ? __half2float(static_cast<const __half*>(out)[e])
+                                                                                         : __bfloat162float(static_cast<const __nv_bfloat16*>(out)[e]);
+}
+// Keys [k0, k1) of sequence s, rows [r0, r1) of its (token, head of the group) list: adds the values that are not finite to the
+// outputs of the rows that see them, as stored in `out` (so null) or in a part so of which row `so_row` is the first.  One warp,
+// after its own stores to these rows.
+template <typename T, int HD>
+__device__ __noinline__ void add_odd_values(const AttnParams& p, int s, int q0, int pos0, int kvh, int k0, int k1, int r0, int r1, float* so, int so_row) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
 #pragma unroll 1
     for (int key = k0; key < k1; ++key) {
-        size_t ko, vo;
-        bool there = true;
+        size_t vo;
         if (p.table) {
-            const int pg = page_of(p, s, key / p.page_size), slot = key % p.page_size;
-            there = pg < p.n_pages;
-            ko = (size_t)pg * p.k_page + (size_t)slot * p.k_row, vo = (size_t)pg * p.v_page + (size_t)slot * p.v_row;
+            const int pg = page_of(p, s, key / p.page_size);
+            if (pg >= p.n_pages) continue;
+            vo = (size_t)pg * p.v_page + (size_t)(key % p.page_size) * p.v_row;
         } else {
-            ko = (size_t)(q0 + key) * p.k_row, vo = (size_t)(q0 + key) * p.v_row;
+            vo = (size_t)(q0 + key) * p.v_row;
         }
-        const T* kr = static_cast<const T*>(p.k) + ko + (size_t)kvh * HD;
         const T* vr = static_cast<const T*>(p.v) + vo + (size_t)kvh * HD;
-        float d = 0.f;
-        if (there) {
+        float v[HD / 32];
+        bool odd = false;
 #pragma unroll
-            for (int j = 0; j < HD / 32; ++j) d += qv[j] * to_f32<T>(kr[lane + 32 * j]);
+        for (int j = 0; j < HD / 32; ++j) v[j] = to_f32<T>(vr[lane + 32 * j]), odd |= v[j] * 0.f != 0.f;
+        if (!__any_sync(0xffffffffu, odd)) continue;
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) {
+            const int tok = r / p.group, pos = pos0 + tok;
+            if (key > pos || (p.window && key <= pos - p.window)) continue;
+            const size_t e = (size_t)(q0 + tok) * p.out_stride + (size_t)(kvh * p.group + r - tok * p.group) * HD + lane;
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) {
+                if (v[j] * 0.f == 0.f) continue;
+                if (so) so[(size_t)(r - so_row) * HD + lane + 32 * j] += v[j];
+                else store_out1(p.out, p.out_dtype, e + 32 * j, load_out1(p.out, p.out_dtype, e + 32 * j) + v[j]);
+            }
         }
-        d = warp_sum(d);
-        const float mn = fmaxf(m, d), mu = mn == -INFINITY ? 0.f : mn;
-        const float f = fast_exp2((m - mu) * p.scale_log2), e = fast_exp2((d - mu) * p.scale_log2);
-        m = mn;
-        l = l * f + e;
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) o[j] = o[j] * f + (there ? e * to_f32<T>(vr[lane + 32 * j]) : 0.f);
     }
 }
 

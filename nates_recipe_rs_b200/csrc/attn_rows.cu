@@ -38,8 +38,7 @@ struct ArSeg {
     int r0, n_rows;       // rows r0 .. + n_rows of the sequence's (token, head of the group) list
     int t0, t1;           // tiles [t0, t1) that hold keys of the rows
     int st0, st1;         // tiles of the segment before that cut
-    int a2, b2;           // keys [a2, b2) are seen by every row
-    int c0;               // first key that is loaded
+    int a, b, a2, b2;     // keys [a, b) are seen by some row, [a2, b2) by all
     int begins, ends;     // the item's first / last segment
     int more;             // tiles of the item after the segment
 };
@@ -50,7 +49,7 @@ struct __align__(16) ArHeader {
     long long scan[36];
     float ml[4][16][2];
     AttnParams p;  // a copy: functions that are not inlined would fetch the kernel's parameters from far away, one by one
-    int abort_flag;
+    int abort_flag, odd;
 };
 
 template <int HD> constexpr size_t ar_smem_bytes() {
@@ -81,12 +80,6 @@ __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
 }
 __device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// a barrier of the math warps that tells all of them whether `x` holds for any thread
-__device__ __forceinline__ bool bar_any(bool x) {
-    int r;
-    asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %1, 0; barrier.cta.red.or.pred.aligned q, 1, 128, p; selp.b32 %0, 1, 0, q; }" : "=r"(r) : "r"((int)x) : "memory");
-    return r != 0;
 }
 __device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
@@ -130,7 +123,7 @@ struct ArWalker {
         g.r0 = rb * AR_ROWS, g.n_rows = min(AR_ROWS, si.q_len * p.group - g.r0);
         const KeyRange kr = key_range(p, si, g.r0 / p.group, (g.r0 + g.n_rows - 1) / p.group + 1);
         g.t0 = max(g.st0, kr.a / AR_TILE), g.t1 = min(g.st1, (kr.b + AR_TILE - 1) / AR_TILE);
-        g.a2 = kr.a2, g.b2 = kr.b2, g.c0 = (kr.a >> p.box_shift) << p.box_shift;
+        g.a = kr.a, g.b = kr.b, g.a2 = kr.a2, g.b2 = kr.b2;
         return true;
     }
 };
@@ -197,7 +190,7 @@ __global__ void __launch_bounds__(AR_THREADS, ArShape<HD>::CTAS_PER_SM) attn_row
         for (int i = 0; i < Sh::STAGES; ++i) mbar_init(smem_u32(&hdr->full[i]), 1), mbar_init(smem_u32(&hdr->empty[i]), 4);
         for (int i = 0; i < AR_SEGS; ++i) mbar_init(smem_u32(&hdr->seg_full[i]), 1), mbar_init(smem_u32(&hdr->seg_empty[i]), 4);
         mbar_init(smem_u32(&hdr->q_full), 1), mbar_init(smem_u32(&hdr->q_empty), 4);
-        hdr->abort_flag = 0;
+        hdr->abort_flag = 0, hdr->odd = 0;
         mbar_fence_init();
     }
     if (tid < (int)(sizeof(AttnParams) / 4)) reinterpret_cast<uint32_t*>(&hdr->p)[tid] = reinterpret_cast<const uint32_t*>(&params)[tid];
@@ -252,14 +245,14 @@ __global__ void __launch_bounds__(AR_THREADS, ArShape<HD>::CTAS_PER_SM) attn_row
             }
             int first, count, slots = 0, pages = 0;
             if (g.t0 < g.t1) {
-                tile_boxes<AR_TILE>(p, g.t0, g.c0, g.kv, first, count);
+                tile_boxes<AR_TILE>(p, g.t0, g.a, g.b, first, count);
                 pages = page_of_boxes<AR_TILE>(p, g.s, g.q0, g.t0, first, count, slots);
             }
             for (int t = g.t0; t < g.t1; ++t, ++it) {
                 const int st = it % Sh::STAGES;
                 int nfirst = 0, ncount = 0, npages = 0, nslots = 0;
                 if (t + 1 < g.t1) {  // the next tile's pages are looked up before this tile's turn comes
-                    tile_boxes<AR_TILE>(p, t + 1, g.c0, g.kv, nfirst, ncount);
+                    tile_boxes<AR_TILE>(p, t + 1, g.a, g.b, nfirst, ncount);
                     npages = page_of_boxes<AR_TILE>(p, g.s, g.q0, t + 1, nfirst, ncount, nslots);
                 }
                 if (it >= Sh::STAGES && !wait_bar(&hdr->empty[st], ((it / Sh::STAGES) - 1) & 1, DEV_TIMEOUT_EMPTY, cta_abort)) break;
@@ -298,7 +291,7 @@ __global__ void __launch_bounds__(AR_THREADS, ArShape<HD>::CTAS_PER_SM) attn_row
         math_sync();  // (also: the buffer of the segment before has been read)
         const ArSeg& w = hdr->seg[sn % AR_SEGS];
         if (!w.valid) break;
-        const int n_rows = w.n_rows, t0 = w.t0, t1 = w.t1, r0 = w.r0, pos0 = w.kv - w.q_len, kv_len = w.kv;
+        const int n_rows = w.n_rows, t0 = w.t0, t1 = w.t1, r0 = w.r0, pos0 = w.kv - w.q_len;
         wait_bar(&hdr->q_full, sn & 1, DEV_TIMEOUT_FULL, cta_abort);
         // this thread's two rows: the keys [lo, hi) they see
         int lo[2], hi[2];
@@ -328,13 +321,16 @@ __global__ void __launch_bounds__(AR_THREADS, ArShape<HD>::CTAS_PER_SM) attn_row
             const uint32_t ks = ring + (uint32_t)st * 2 * Sh::TILE_BYTES, vs = ks + Sh::TILE_BYTES;
             const int k0 = t * AR_TILE;
             const bool masked = k0 < w.a2 || k0 + AR_TILE > w.b2;  // some row does not see some key of the tile
-            const int c0 = w.c0 - k0, c1 = kv_len - k0;  // keys of the tile outside [c0, c1): not loaded
-            if (c0 > 0 || c1 < AR_TILE) {
+            if (masked) {
                 uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)st * 2 * Sh::TILE_BYTES + Sh::TILE_BYTES);
-                for (int i = tid; i < Sh::NCH * AR_TILE * 8; i += 128) {
-                    const int key = (i >> 3) % AR_TILE;
-                    if (key < c0 || key >= c1) vp[i] = make_uint4(0u, 0u, 0u, 0u);
+                const int left = min(max(w.a2 - k0, 0), AR_TILE), right = min(max(w.b2 - k0, left), AR_TILE);
+                bool odd = false;
+#pragma unroll 1
+                for (int ch = 0; ch < Sh::NCH; ++ch) {
+                    if (left > 0) odd |= clear_values<T, 1>(vp + ch * AR_TILE * 8, 0, left, w.a - k0, w.b - k0, tid, 128);
+                    odd |= clear_values<T, 1>(vp + ch * AR_TILE * 8, right, AR_TILE, w.a - k0, w.b - k0, tid, 128);
                 }
+                if (odd) hdr->odd = 1;  // (stays set: the rows of later segments are looked at too)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage is refilled by a copy
                 math_sync();
             }
@@ -435,26 +431,7 @@ __global__ void __launch_bounds__(AR_THREADS, ArShape<HD>::CTAS_PER_SM) attn_row
         auto row_sees = [&](int r) {  // row r has keys at all (else its output is 0)
             return pos0 + (r0 + r) / p.group >= 0;
         };
-        // outputs that are not finite: from a value that the row does not see, or by the formula; either way again, exactly
-        float odd[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) odd[0] += (o[i][0] + o[i][1]) * 0.f, odd[1] += (o[i][2] + o[i][3]) * 0.f;
-        if (bar_any((odd[0] != odd[0] && qr < n_rows) || (odd[1] != odd[1] && qr + 8 < n_rows))) {
-#pragma unroll 1
-            for (int r = warp; r < n_rows; r += 4) {
-                const int tok = (r0 + r) / p.group, pos = pos0 + tok;
-                float em, el, eo[HD / 32];
-                attn_row_exact<T, HD>(p, w.s, w.q0, tok, w.kvh * p.group + (r0 + r) % p.group, w.kvh,
-                                      max(w.st0 * AR_TILE, p.window ? max(0, pos - p.window + 1) : 0), min(w.st1 * AR_TILE, pos + 1), em, el, eo);
-                const float inv = 1.f / el;
-#pragma unroll
-                for (int j = 0; j < HD / 32; ++j) {
-                    if (whole) store_out1(p.out, p.out_dtype, out_elem(r) + lane + 32 * j, row_sees(r) ? eo[j] * inv : 0.f);
-                    else so[(size_t)r * HD + lane + 32 * j] = eo[j];
-                }
-                if (!whole && lane == 0) sml[2 * r] = em, sml[2 * r + 1] = el;
-            }
-        } else {
+        {
             // the four warps' parts, added through one buffer in a fixed order
             if (pq == 0)
 #pragma unroll
@@ -501,6 +478,13 @@ __global__ void __launch_bounds__(AR_THREADS, ArShape<HD>::CTAS_PER_SM) attn_row
                     if (c == 0) sml[2 * r] = mm, sml[2 * r + 1] = ll;
                 }
             }
+        }
+        if (hdr->odd) {  // (set before the barriers above; rows by warp, once all their stores are done)
+            math_sync();
+            const int lo = max(w.a, w.st0 * AR_TILE), hi = min(w.b, w.st1 * AR_TILE), left = min(max(w.a2, lo), hi), right = max(min(w.b2, hi), left);
+            const int ra = r0 + n_rows * warp / 4, rz = r0 + n_rows * (warp + 1) / 4;
+            add_odd_values<T, HD>(p, w.s, w.q0, pos0, w.kvh, lo, left, ra, rz, so, r0);
+            add_odd_values<T, HD>(p, w.s, w.q0, pos0, w.kvh, right, hi, ra, rz, so, r0);
         }
         if (w.begins && !w.ends && tid == 0) {
             // this item goes on in the next CTAs: how many of them

@@ -17,8 +17,8 @@
 // row tile 0 / 1 (an issuing thread blocks while the tensor cores are busy, and every wait or commit costs it some 90 cycles more:
 // with one issuer for both tiles these were idle time of the tensor cores); 17 issues the TMA copies (queries, and keys and values
 // through a ring of 128-key slots); 18 plans: it alone works out which item comes next and hands the others its bounds through
-// shared memory, ahead of time (done by every warp for itself this took each some 4000 cycles per item), and it clears what was not
-// loaded out of the value tiles that need it.
+// shared memory, ahead of time (done by every warp for itself this took each some 4000 cycles per item), and it prepares the value
+// tiles with masked keys.
 // The CTAs stay: each takes items until none is left, so that the copies and the scores of the next item run under the epilogue
 // of the one before (a CTA per item spent 7 us between the last tile of one and the first of the next).
 // Every wait is bounded; on expiry the CTA records a status code, drains its copies, frees its tensor memory and returns.
@@ -53,14 +53,13 @@ struct AtSeg {
     int kvh, tok0, tok1;  // tokens [tok0, tok1) of the sequence
     int t0, t1;         // tiles [t0, t1) that hold keys of its rows
     int st0, st1;       // tiles of the segment before that cut
+    int a, b, a2, b2;   // keys [a, b) are seen by some row, [a2, b2) by all
     int u0, u1;         // tiles [u0, u1) whose keys every row sees
-    int d0, d1;         // tiles [d0, d1) that are loaded whole
-    int a;              // first key that any row sees
     int begins, ends;   // the item's first / last segment
     int more;           // tiles of the item after the segment
 
-    // rows of value tile t were not loaded, or are not of this sequence
-    __device__ __forceinline__ bool dirty(int t) const { return t < d0 || t >= d1; }
+    // some row does not see some key of tile t
+    __device__ __forceinline__ bool masked(int t) const { return t < u0 || t >= u1; }
 };
 
 struct __align__(16) AtHeader {
@@ -70,7 +69,7 @@ struct __align__(16) AtHeader {
     long long scan[36];
     AttnParams p;  // a copy: functions that are not inlined would fetch the kernel's parameters from far away, one by one
     uint32_t tmem_base;
-    int abort_flag;
+    int abort_flag, odd;
 };
 template <int HD> constexpr size_t at_smem_bytes() { return 1024 + (size_t)(2 + AtShape<HD>::SLOTS) * AtShape<HD>::TILE_BYTES + sizeof(AtHeader); }
 
@@ -278,35 +277,12 @@ struct AtWalker {
         g.valid = 1, g.s = s, g.q0 = si.q0, g.q_len = si.q_len, g.kv = si.kv;
         g.tok0 = blk * tb, g.tok1 = min(g.tok0 + tb, si.q_len);
         const KeyRange kr = key_range(p, si, g.tok0, g.tok1);
-        g.a = kr.a;
+        g.a = kr.a, g.b = kr.b, g.a2 = kr.a2, g.b2 = kr.b2;
         g.t0 = max(g.st0, kr.a / AT_TILE), g.t1 = min(g.st1, (kr.b + AT_TILE - 1) / AT_TILE);
         g.u0 = (kr.a2 + AT_TILE - 1) / AT_TILE, g.u1 = kr.b2 / AT_TILE;
-        g.d0 = (((kr.a >> p.box_shift) << p.box_shift) + AT_TILE - 1) / AT_TILE, g.d1 = si.kv / AT_TILE;
         return true;
     }
 };
-
-// The 16 rows of a warp (rows row0 .. row0 + 15 of the row tile whose first token is tok0 of the block) without the tensor cores
-template <typename T, int HD>
-__device__ __noinline__ void at_exact_rows(const AttnParams& p, const AtSeg& w, int tok0, int row0, int tile_rows, bool whole, float* so, float* ml) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll 1
-    for (int row = row0; row < row0 + 16; ++row) {
-        const int tok = w.tok0 + tok0 + row / p.group, pos = w.kv - w.q_len + tok, head = w.kvh * p.group + row % p.group;
-        if (row >= tile_rows || tok >= w.tok1) break;
-        float m, l, o[HD / 32];
-        attn_row_exact<T, HD>(p, w.s, w.q0, tok, head, w.kvh, max(w.st0 * AT_TILE, p.window ? max(0, pos - p.window + 1) : 0),
-                              min(w.st1 * AT_TILE, pos + 1), m, l, o);
-        const int r = (tok - w.tok0) * p.group + row % p.group;
-        const float inv = 1.f / l;
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-            if (whole) store_out1(p.out, p.out_dtype, (size_t)(w.q0 + tok) * p.out_stride + (size_t)head * HD + lane + 32 * j, pos >= 0 ? o[j] * inv : 0.f);
-            else so[(size_t)r * HD + lane + 32 * j] = o[j];
-        }
-        if (!whole && lane == 0) ml[2 * r] = m, ml[2 * r + 1] = l;
-    }
-}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -333,7 +309,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
             mbar_init(smem_u32(&hdr->p_part[i]), 8), mbar_init(smem_u32(&hdr->p_full[i]), 8);
             for (int j = 0; j < 4; ++j) mbar_init(smem_u32(&hdr->turn[i][j]), 2);
         }
-        hdr->abort_flag = 0;
+        hdr->abort_flag = 0, hdr->odd = 0;
         mbar_fence_init();
     }
     if (warp == Sh::MMA0) {
@@ -397,7 +373,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                 }
             }
         }
-        // It also clears the rows that were not loaded out of the value tiles (the tensor cores would add 0 * whatever was there):
+        // It also prepares the value tiles with keys that some row does not see (clear_values: the tensor cores add 0 * v there),
         // those of a segment after the next one is laid down.  The issuers ask for each such tile when it has landed and wait for
         // it before they ask for the next: this warp does not follow the ring's own barriers, most of whose phases it would skip.
         if (!any) {  // nothing to do for this CTA
@@ -423,20 +399,22 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
             const int tiles = max(last.t1 - last.t0, 0);
             for (int k = 0; k < tiles; ++k) {
                 const int t = last.t0 + k;
-                if (!last.dirty(t)) continue;
+                if (!last.masked(t)) continue;
                 if (!wait(&hdr->v_ask, n_v++, DEV_TIMEOUT_FULL)) {
                     ok = false;
                     break;
                 }
-                const int c0 = min(max(((last.a >> p.box_shift) << p.box_shift) - t * AT_TILE, 0), AT_TILE), c1 = max(min(last.kv - t * AT_TILE, AT_TILE), c0);
+                const int k0 = t * AT_TILE, left = min(max(last.a2 - k0, 0), AT_TILE), right = min(max(last.b2 - k0, left), AT_TILE);
+                bool odd = false;
                 // order of the slots: K0 V0 K1 V1 ..., or (scores one tile ahead) K0 K1 V0 K2 V1 ...
                 const int v_it = it + (Sh::WIDE ? 2 * (min(k + 2, tiles) + k) : 2 * k + 1);
 #pragma unroll 1
                 for (int ch = 0; ch < Sh::NCH * Sh::HALVES; ++ch) {
                     uint4* vp = reinterpret_cast<uint4*>(sm + (size_t)(2 + (v_it + ch / Sh::NCH) % Sh::SLOTS) * Sh::TILE_BYTES) + (ch % Sh::NCH) * AT_TILE * 8;
-                    for (int i = lane; i < c0 * 8; i += 32) vp[i] = make_uint4(0u, 0u, 0u, 0u);
-                    for (int i = c1 * 8 + lane; i < AT_TILE * 8; i += 32) vp[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (left > 0) odd |= clear_values<T, 8>(vp, 0, left, last.a - k0, last.b - k0, lane, 32);
+                    odd |= clear_values<T, 8>(vp, right, AT_TILE, last.a - k0, last.b - k0, lane, 32);
                 }
+                if (odd) *reinterpret_cast<volatile int*>(&hdr->odd) = 1;  // (stays set: the rows of later segments are looked at too)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read by the tensor cores, refilled by a copy
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ok));
@@ -450,11 +428,11 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
         bool ok = true;
         for (int n = 0; ok && have_seg(n); done_seg(n), ++n) {
             const AtSeg& w = hdr->seg[n % AT_SEGS];
-            const int t0 = w.t0, t1 = w.t1, kvh = w.kvh, q0 = w.q0, kv_len = w.kv;
+            const int t0 = w.t0, t1 = w.t1, kvh = w.kvh, q0 = w.q0;
             if (t0 >= t1) continue;
             const int nq = Sh::WIDE || w.tok1 - w.tok0 > tpt ? 2 : 1;
             int first, cnt, pages, slots;
-            tile_boxes<AT_TILE>(p, t0, w.a, kv_len, first, cnt);
+            tile_boxes<AT_TILE>(p, t0, w.a, w.b, first, cnt);
             pages = page_of_boxes<AT_TILE>(p, w.s, q0, t0, first, cnt, slots);
             if (q_no > 0 && !wait(&hdr->q_empty, q_no - 1, DEV_TIMEOUT_EMPTY)) break;
             if (lane == 0) mbar_arrive_expect_tx(smem_u32(&hdr->q_full), (uint32_t)(nq * Sh::NCH * tile_rows * 128));
@@ -480,7 +458,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
             for (int t = t0; t < t1 && ok; ++t) {
                 int nfirst = 0, ncnt = 0, npages = 0, nslots = 0;
                 if (t + 1 < t1) {  // the next tile's pages are looked up before its turn comes
-                    tile_boxes<AT_TILE>(p, t + 1, w.a, kv_len, nfirst, ncnt);
+                    tile_boxes<AT_TILE>(p, t + 1, w.a, w.b, nfirst, ncnt);
                     npages = page_of_boxes<AT_TILE>(p, w.s, q0, t + 1, nfirst, ncnt, nslots);
                 }
                 if (Sh::WIDE) {
@@ -537,7 +515,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
         };
         for (int n = 0; ok && have_seg(n); done_seg(n), ++n) {
             const AtSeg& w = hdr->seg[n % AT_SEGS];
-            const int t0 = w.t0, t1 = w.t1, d0 = w.d0, d1 = w.d1;
+            const int t0 = w.t0, t1 = w.t1, u0 = w.u0, u1 = w.u1;
             if (t0 >= t1) continue;
             if (!wait(&hdr->q_full, q_no, DEV_TIMEOUT_FULL)) break;
             ++q_no;
@@ -546,7 +524,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
             for (int t = t0; t < t1 && ok; ++t, ++j) {
                 const int s0 = it % Sh::SLOTS, s1 = (it + 1) % Sh::SLOTS;
                 ok = wait(&hdr->full[s0], it / Sh::SLOTS, DEV_TIMEOUT_FULL) && wait(&hdr->full[s1], (it + 1) / Sh::SLOTS, DEV_TIMEOUT_FULL);
-                if (ok && (t < d0 || t >= d1)) {  // rows that were not loaded are cleared by the planning warp
+                if (ok && (t < u0 || t >= u1)) {  // keys that some row does not see: prepared by the planning warp
                     if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ask));
                     ok = wait(&hdr->v_ok, n_v++, DEV_TIMEOUT_FULL);
                 }
@@ -555,12 +533,12 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        for (int h = 0; h < 2; ++h) {
-                            const uint64_t vd = umma_desc_v(ring + (uint32_t)(h ? s1 : s0) * Sh::TILE_BYTES);
+                        const uint64_t v0 = umma_desc_v(ring + (uint32_t)s0 * Sh::TILE_BYTES), v1 = umma_desc_v(ring + (uint32_t)s1 * Sh::TILE_BYTES);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                umma_ts(tmem + AT_COL_O + 128u * h, tmem + AT_COL_S + 128u * (j & 1) + AT_COL_P + 8u * (4 * part + k), vd + (uint64_t)((4 * part + k) * (2048 >> 4)),
-                                        Sh::IDESC_O(BF16), t > t0 || part == 0 || k > 0);
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t pt = tmem + AT_COL_S + 128u * (j & 1) + AT_COL_P + 8u * (4 * part + k), acc = t > t0 || part == 0 || k > 0;
+                            umma_ts(tmem + AT_COL_O, pt, v0 + (uint64_t)((4 * part + k) * (2048 >> 4)), Sh::IDESC_O(BF16), acc);
+                            umma_ts(tmem + AT_COL_O + 128u, pt, v1 + (uint64_t)((4 * part + k) * (2048 >> 4)), Sh::IDESC_O(BF16), acc);
                         }
                     }
                 }
@@ -619,9 +597,9 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                 else mbar_arrive(smem_u32(bar));
             }
         };
-        // a value tile with rows that were not loaded goes through the planning warp while its scores are in softmax
-        auto ask_v = [&](bool dirty, int v_it) {
-            if (!dirty) return true;
+        // a value tile with keys that some row does not see goes through the planning warp while its scores are in softmax
+        auto ask_v = [&](bool masked, int v_it) {
+            if (!masked) return true;
             if (!wait(&hdr->full[v_it % Sh::SLOTS], v_it / Sh::SLOTS, DEV_TIMEOUT_FULL)) return false;
             if (lane == 0) mbar_arrive(smem_u32(&hdr->v_ask));
             ++n_v;
@@ -629,7 +607,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
         };
         for (int n = 0; ok && have_seg(n); done_seg(n), ++n) {
             const AtSeg& w = hdr->seg[n % AT_SEGS];
-            const int t0 = w.t0, t1 = w.t1, d0 = w.d0, d1 = w.d1;
+            const int t0 = w.t0, t1 = w.t1, u0 = w.u0, u1 = w.u1;
             if (t0 >= t1) continue;
             active = i == 0 || w.tok1 - w.tok0 > tpt;
             int sl = it % Sh::SLOTS;
@@ -640,12 +618,12 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
             release(&hdr->empty[sl]);
             if (t0 + 1 == t1) release(&hdr->q_empty);
             ++it;
-            ok = ask_v(t0 < d0 || t0 >= d1, it);
+            ok = ask_v(t0 < u0 || t0 >= u1, it);
             for (int t = t0; t < t1 && ok; ++t) {
                 const int vs = it % Sh::SLOTS, ks = (it + 1) % Sh::SLOTS;
                 const bool more = t + 1 < t1;
                 ok = wait(&hdr->full[vs], it / Sh::SLOTS, DEV_TIMEOUT_FULL);
-                if (ok && (t < d0 || t >= d1)) ok = wait(&hdr->v_ok, n_v - 1, DEV_TIMEOUT_FULL);
+                if (ok && (t < u0 || t >= u1)) ok = wait(&hdr->v_ok, n_v - 1, DEV_TIMEOUT_FULL);
                 if (ok && more) ok = wait(&hdr->full[ks], (it + 1) / Sh::SLOTS, DEV_TIMEOUT_FULL);
                 if (ok && active) {
                     ok = wait(&hdr->p_part[i], n_p, DEV_TIMEOUT_MMA);
@@ -669,7 +647,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                     if (t + 2 == t1) release(&hdr->q_empty);
                 }
                 it += more ? 2 : 1;
-                if (more) ok = ask_v(t + 1 < d0 || t + 1 >= d1, it);
+                if (more) ok = ask_v(t + 1 < u0 || t + 1 >= u1, it);
             }
         }
         __syncwarp();
@@ -809,7 +787,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                 // each lane its own columns, 8 or 4 bytes a time (turning them within the four lanes of a row for wider stores took
                 // three times the instructions, which are what bounds this part)
                 char* dst[2];
-                uint64_t inv[2], odd[2] = {0ull, 0ull};
+                uint64_t inv[2];
                 bool live[2];
                 const bool f32 = !whole || p.out_dtype == QMM_DT_F32, f16 = p.out_dtype == QMM_DT_F16;
 #pragma unroll
@@ -839,7 +817,6 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint64_t x = f32x2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
-                        odd[j & 1] = fma2(x, 0ull, odd[j & 1]);  // 0 * x is 0, or NaN where x is not finite
                         v[j] = mul2(x, inv[j & 1]);
                     }
                     if (f32) {
@@ -860,10 +837,13 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                             if (live[j & 1]) *reinterpret_cast<uint32_t*>(dst[j & 1] + (32 * q + 8 * (j >> 1)) * 2) = h[j];
                     }
                 }
-                // outputs that are not finite: from a value that the row does not see, or by the formula; either way again, exactly
-                const float odd0 = lo2(odd[0]) + hi2(odd[0]), odd1 = lo2(odd[1]) + hi2(odd[1]);
-                if (__any_sync(0xffffffffu, (live[0] && odd0 != odd0) || (live[1] && odd1 != odd1)))
-                    at_exact_rows<T, HD>(p, w, wg * tpt, row0 - (lane >> 2), tile_rows, whole, so, ml);
+                if (*reinterpret_cast<volatile int*>(&hdr->odd)) {
+                    const int lo_k = max(w.a, w.st0 * AT_TILE), hi_k = min(w.b, w.st1 * AT_TILE), left = min(max(w.a2, lo_k), hi_k), right = max(min(w.b2, hi_k), left);
+                    // the warp's rows of the item
+                    const int base = w.tok0 * p.group, first = wg * tile_rows + row0 - (lane >> 2), end = min(min(first + 16, (wg + 1) * tile_rows), n_tok * p.group);
+                    add_odd_values<T, HD>(p, w.s, w.q0, pos0, w.kvh, lo_k, left, base + first, base + end, so, base);
+                    add_odd_values<T, HD>(p, w.s, w.q0, pos0, w.kvh, right, hi_k, base + first, base + end, so, base);
+                }
             }
             if (w.begins && !w.ends && tid == 0) {  // this item goes on in the next CTAs: how many of them
                 ArJoin j;
