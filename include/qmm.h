@@ -340,8 +340,9 @@ int launch_attn_prefill_f16kv_at(const float* q, const void* k16, const void* v1
  * launch_attn_packed: the same without a cache, for whole prompts: the keys and values are rows of the batch (kv_len and max_kv
  *   unused; k and v in q's type, rows k_stride / v_stride elements apart, multiples of 8), so row i of a sequence sees rows 0..i
  *   of it.
- * Products run on the tensor cores with f32 accumulation; the probabilities are rounded to the type of v.  Bit-identical
- * across reruns. */
+ * Products run on the tensor cores with f32 accumulation; the probabilities (scaled to at most 256) are rounded to the type of v,
+ * and their sum with the values is an f32 before it is divided: values of a bf16 cache above about 1e30 may overflow it.
+ * Bit-identical across reruns. */
 #define QMM_DT_F32 0
 #define QMM_DT_F16 1
 #define QMM_DT_BF16 2

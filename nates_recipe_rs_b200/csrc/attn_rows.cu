@@ -1,5 +1,5 @@
-// Attention of one or a few new tokens per sequence over a paged cache (decode) on mma.sync.  The counterpart, for a batch of sequences of different lengths, of the upstream's gpu_gqa_attn_into
-// (gpu-core/src/infer_ops.rs:160-189).
+// Attention of one or a few new tokens per sequence over a paged cache (decode) on mma.sync.  The counterpart, for a batch of
+// sequences of different lengths, of the upstream's gpu_gqa_attn_into (gpu-core/src/infer_ops.rs:160-189).
 //
 //   out[r, h] = sum_t w_t V_t / sum_t w_t,  w_t = exp(kq_scale * q_r . K_t - max),  t in (pos_r - window, pos_r]
 //
@@ -12,6 +12,8 @@
 // scratch as (maximum, sum, unnormalised output) and attn_join_kernel adds them in key order, so reruns are bit identical.
 // q, k, v are f16 or bf16; the probabilities are rounded to the same type for the second product (tensor-core operands),
 // scores, maximum, sum and output stay f32.
+// Measured: 64 sequences of 91 to 8192 keys, 64/8 heads of 128, bf16: 104 us, 5.4 TB/s of cache; one sequence of 131001 keys,
+// 32/8 heads: 92 us, 5.8 TB/s; one of 2048: 12.9 us, of which the first copy is under way after 4 and the joining takes 3.
 #include "attn_pages.cuh"
 
 namespace qmm {
@@ -509,70 +511,71 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     constexpr int E = HD / 32, BATCH = 8;  // elements of a lane: E lane .. E lane + E - 1
     pdl_wait_prior_grids();
     const ArJoin j = reinterpret_cast<const ArJoin*>(p.scratch)[blockIdx.x];
-    const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (r >= j.n_rows) return;
-    auto slot_of = [&](int i) { return 2 * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0); };
-    auto load = [&](int i, float (&x)[E]) {
-        const float* o = ArScratch<HD, R>::o(p.scratch, ctas, slot_of(i)) + (size_t)r * HD + E * lane;
-        if constexpr (E % 4 == 0) {
+    const int lane = threadIdx.x & 31;
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < j.n_rows; r += gridDim.y * 4) {
+        auto slot_of = [&](int i) { return 2 * ((int)blockIdx.x + i) + (i == 0 ? 1 : 0); };
+        auto load = [&](int i, float (&x)[E]) {
+            const float* o = ArScratch<HD, R>::o(p.scratch, ctas, slot_of(i)) + (size_t)r * HD + E * lane;
+            if constexpr (E % 4 == 0) {
 #pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(o + e);
-                x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
+                for (int e = 0; e < E; e += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(o + e);
+                    x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
+                }
+            } else if constexpr (E == 2) {
+                const float2 v = *reinterpret_cast<const float2*>(o);
+                x[0] = v.x, x[1] = v.y;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = o[e];
             }
-        } else if constexpr (E == 2) {
-            const float2 v = *reinterpret_cast<const float2*>(o);
-            x[0] = v.x, x[1] = v.y;
-        } else {
+        };
+        float x[BATCH][E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = o[e];
-        }
-    };
-    float x[BATCH][E];
+        for (int i = 0; i < BATCH; ++i)
+            if (i < j.n_parts) load(i, x[i]);
+        float mm = -INFINITY;
+        for (int i = lane; i < j.n_parts; i += 32) mm = fmaxf(mm, ArScratch<HD, R>::ml(p.scratch, ctas, slot_of(i))[2 * r]);
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i)
-        if (i < j.n_parts) load(i, x[i]);
-    float mm = -INFINITY;
-    for (int i = lane; i < j.n_parts; i += 32) mm = fmaxf(mm, ArScratch<HD, R>::ml(p.scratch, ctas, slot_of(i))[2 * r]);
+        for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+        const float mu = mm == -INFINITY ? 0.f : mm;
+        float ll = 0.f, acc[E];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    const float mu = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int i0 = 0; i0 < j.n_parts; i0 += 32) {
-        float f = 0.f, lp = 0.f;
-        if (i0 + lane < j.n_parts) {
-            const float* ml = ArScratch<HD, R>::ml(p.scratch, ctas, slot_of(i0 + lane)) + 2 * r;
-            f = fast_exp2((ml[0] - mu) * p.scale_log2);  // (a part without keys: maximum -inf, sum 0; its factor of 0 keeps both)
-            lp = ml[1] * f;
-        }
-        const int n = min(32, j.n_parts - i0);
-        for (int b = 0; b < n; b += BATCH) {
-            float y[BATCH][E];
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) y[i][e] = x[i][e];
-                if (i0 + b + BATCH + i < j.n_parts) load(i0 + b + BATCH + i, x[i]);  // the next batch
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+        for (int i0 = 0; i0 < j.n_parts; i0 += 32) {
+            float f = 0.f, lp = 0.f;
+            if (i0 + lane < j.n_parts) {
+                const float* ml = ArScratch<HD, R>::ml(p.scratch, ctas, slot_of(i0 + lane)) + 2 * r;
+                f = fast_exp2((ml[0] - mu) * p.scale_log2);  // (a part without keys: maximum -inf, sum 0; its factor of 0 keeps both)
+                lp = ml[1] * f;
             }
+            const int n = min(32, j.n_parts - i0);
+            for (int b = 0; b < n; b += BATCH) {
+                float y[BATCH][E];
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const float fi = __shfl_sync(0xffffffffu, f, b + i), li = __shfl_sync(0xffffffffu, lp, b + i);
-                if (b + i < n) {
-                    ll += li;
+                for (int i = 0; i < BATCH; ++i) {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += y[i][e] * fi;
+                    for (int e = 0; e < E; ++e) y[i][e] = x[i][e];
+                    if (i0 + b + BATCH + i < j.n_parts) load(i0 + b + BATCH + i, x[i]);  // the next batch
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const float fi = __shfl_sync(0xffffffffu, f, b + i), li = __shfl_sync(0xffffffffu, lp, b + i);
+                    if (b + i < n) {
+                        ll += li;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) acc[e] += y[i][e] * fi;
+                    }
                 }
             }
         }
-    }
-    const int tok = (j.tok_row0 + r) / p.group, h = j.kvh * p.group + (j.tok_row0 + r) % p.group;
-    const bool sees = j.any_key + tok >= 0;
-    const float inv = 1.f / ll;
+        const int tok = (j.tok_row0 + r) / p.group, h = j.kvh * p.group + (j.tok_row0 + r) % p.group;
+        const bool sees = j.any_key + tok >= 0;
+        const float inv = 1.f / ll;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        store_out1(p.out, p.out_dtype, (size_t)(j.q0 + tok) * p.out_stride + (size_t)h * HD + E * lane + e, sees ? acc[e] * inv : 0.f);
+        for (int e = 0; e < E; ++e)
+            store_out1(p.out, p.out_dtype, (size_t)(j.q0 + tok) * p.out_stride + (size_t)h * HD + E * lane + e, sees ? acc[e] * inv : 0.f);
+    }
 }
 
 // ---- host side ----

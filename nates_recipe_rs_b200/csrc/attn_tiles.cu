@@ -9,7 +9,10 @@
 //     O += P V     128 x HD x 128, P from tensor memory, V from shared memory as it arrives (keys are the K dimension: the
 //                  operand is "MN major"), O in tensor memory for the whole run over the keys
 // While the threads of one row tile compute exponentials the tensor cores work for the other: the two pipes (16 exponentials per
-// clock and SM; 8192 flops) need about the same time at HD = 128.  The running maximum that P is scaled by is only moved when a
+// clock and SM; 8192 flops) need about the same time at HD = 128, 2048 cycles per tile of keys, and so does shared memory (the
+// operands of S = Q K^T alone take its whole bandwidth).  A step takes about 3600 cycles: scores, softmax and outputs of ONE row
+// tile follow one another, and the turns (below) leave gaps.  Measured: 8192 tokens, 32/8 heads of 128, causal: 520 us alone on an
+// idle GPU, 1060 TFLOP/s of the products that are not masked; 4096 tokens 166 us; profiles/attn_paged.md.  The running maximum that P is scaled by is only moved when a
 // row's maximum has grown by more than 2^8 (P <= 256 fits f16, l and O are f32): O is rescaled in tensor memory a few times per
 // run instead of once per tile, with no separate correction step.
 // Warps: 0-7 and 8-15 softmax of row tile 0 / 1 (and its epilogue), 16 rows each, a row in four lanes: with a thread per row, four
@@ -43,7 +46,7 @@ template <int HD> struct AtShape {
     __host__ __device__ static constexpr uint32_t IDESC_O(bool bf16) { return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((HD / HALVES >> 3) << 17) | ((128 >> 4) << 24); }
 };
 // tensor memory columns: S of tile i at 128 i, P over the second half of S (the half that is read last goes there first), O of
-// tile i at 256 + 128 i
+// tile i at 256 + 128 i (wide heads: S of the even and odd tiles of keys at 0 and 128, O at 256)
 constexpr uint32_t AT_COL_S = 0, AT_COL_P = 64, AT_COL_O = 256;
 
 // A segment: some of the key tiles of an item, as the planning warp hands it to the others
@@ -743,8 +746,9 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                     }
                 }
                 // The two row tiles take turns at the exponentials: left to themselves both wait for scores at the same time and then
-                // share the special-function units, while the tensor cores idle (8192 tokens, 32/8 heads: 619 us without turns, 550 with;
-                // per scheduler, warp & 3: whoever is ready there goes on)
+                // share the special-function units, while the tensor cores idle (8192 tokens, 32/8 heads, when the turns were added:
+                // 619 us without, 550 with; handed over after half of the keys: 633; a quarter of the exponentials as polynomials
+                // instead: slower, the schedulers' issue slots bound it then).  Per scheduler, warp & 3: whoever is ready there goes on
                 if (both) {
                     if ((wg == 1 || n_turn > 0) && !wait(&hdr->turn[wg][warp & 3], wg == 1 ? n_turn : n_turn - 1, DEV_TIMEOUT_MMA)) {
                         ok = false;
