@@ -12,7 +12,7 @@
 // clock and SM; 8192 flops) need about the same time at HD = 128, 2048 cycles per tile of keys, and so does shared memory (the
 // operands of S = Q K^T alone take its whole bandwidth).  A step takes about 3600 cycles: scores, softmax and outputs of ONE row
 // tile follow one another, and the turns (below) leave gaps.  Measured: 8192 tokens, 32/8 heads of 128, causal: 520 us alone on an
-// idle GPU, 1060 TFLOP/s of the products that are not masked; 4096 tokens 166 us; profiles/attn_paged.md.  The running maximum that P is scaled by is only moved when a
+// idle GPU, 1060 TFLOP/s of the products that are not masked; 4096 tokens 166 us.  The running maximum that P is scaled by is only moved when a
 // row's maximum has grown by more than 2^8 (P <= 256 fits f16, l and O are f32): O is rescaled in tensor memory a few times per
 // run instead of once per tile, with no separate correction step.
 // Warps: 0-7 and 8-15 softmax of row tile 0 / 1 (and its epilogue), 16 rows each, a row in four lanes: with a thread per row, four
@@ -715,7 +715,8 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                 for (int e = 0; e < 2; ++e) {
                     mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 1));
                     mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 2));
-                    grew |= (mt[e] - m[e]) * c > 8.f || (m[e] == -INFINITY && mt[e] > -INFINITY);
+                    // (rows that are none, hi 0, hold anything: they have no say, or reruns would not be bit identical)
+                    grew |= hi[e] > 0 && ((mt[e] - m[e]) * c > 8.f || (m[e] == -INFINITY && mt[e] > -INFINITY));
                 }
                 bool o_done = !Sh::WIDE || t == t0;  // the outputs so far are complete (two row tiles: they are when the scores are)
                 if (t == t0) {

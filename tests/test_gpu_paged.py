@@ -200,6 +200,17 @@ def test_reruns_are_bit_identical(ops):
             assert torch.equal(one, paged(ops, b))
 
 
+@pytest.mark.parametrize("nqh,nkv", [(66, 2), (10, 2), (71, 1)])
+def test_reruns_with_groups_that_leave_rows_unused(ops, nqh, nkv):
+    """A group that does not divide a tile of rows leaves rows of it unused, whose shared memory holds anything."""
+    nqh -= nqh % nkv + (7 if nqh == 71 else 0)
+    b = ref.Batch([40 - i % 40 for i in range(130)], [300 - i for i in range(130)], nqh, nkv, 96, 256, BF16, seed=16)
+    one = check(ops, b)
+    for hd in (64, 128, 96):  # other kernels leave other contents behind
+        paged(ops, ref.Batch([100], [700], 8, 2, hd, 16, F16, seed=hd, values=1e4))
+        assert torch.equal(one, paged(ops, b))
+
+
 def test_a_sequence_does_not_depend_on_its_neighbours_values(ops):
     b = ref.Batch([40, 40, 1], [200, 300, 90], 8, 2, 128, 16, F16, seed=14)
     one = paged(ops, b)
