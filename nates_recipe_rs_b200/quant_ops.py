@@ -448,8 +448,8 @@ def gpu_gqa_attn_paged_into(q, kpages, vpages, page_table, cu_q, kv_len, out, nq
         raise TypeError("q must have the cache's type, out be float32, float16 or bfloat16")
     if scratch is None:
         scratch = gpu_gqa_attn_paged_scratch(q, kpages, kv_len, nqh, max_q, max_kv)
-    elif scratch.get_device() != index:
-        raise ValueError(f"scratch: expected a tensor on cuda:{index}")
+    elif scratch.get_device() != index or not scratch.is_contiguous():  # (its bytes are counted from its elements)
+        raise ValueError(f"scratch: expected a contiguous tensor on cuda:{index}")
     batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), _int32(kv_len, n_seqs, index, "kv_len"), n_seqs, total, max_q, max_kv)
     _launch_on(index, "launch_attn_paged", q.data_ptr(), q_stride, kv, batch, out.data_ptr(), _DT[out.dtype], o_stride, scratch.data_ptr(),
                scratch.numel() * scratch.element_size(), nqh, window, kq_scale)

@@ -1,0 +1,48 @@
+"""The Python forms of the paged-cache operators without a GPU: what they refuse, and what they hand to the library.  Tensors in
+host memory pass for tensors of device 0, and the launch is recorded instead of made."""
+import pytest
+import torch
+
+from nates_recipe_rs_b200 import quant_ops as ops
+
+F16, I32 = torch.float16, torch.int32
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    calls = []
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    monkeypatch.setattr(ops, "_launch_on", lambda index, name, *args: calls.append((name, args)))
+    return calls
+
+
+def batch(**kw):
+    d = dict(q=torch.zeros(3, 8 * 64, dtype=F16), kpages=torch.zeros(6, 16, 2, 64, dtype=F16), vpages=torch.zeros(6, 16, 2, 64, dtype=F16),
+             page_table=torch.zeros(2, 3, dtype=I32), cu_q=torch.zeros(3, dtype=I32), kv_len=torch.zeros(2, dtype=I32), out=torch.zeros(3, 8 * 64),
+             scratch=torch.empty(4096, dtype=torch.uint8), nqh=8, max_q=2, max_kv=30)
+    d.update(kw)
+    return d
+
+
+def attn(**kw):
+    ops.gpu_gqa_attn_paged_into(**batch(**kw))
+
+
+def append(**kw):
+    d = batch(**{"out": torch.zeros(3, 8 * 64, dtype=F16), **kw})
+    ops.gpu_rope_kv_append_paged_into(d.get("qkv", torch.zeros(3, 12 * 64)), d["out"], d["kpages"], d["vpages"], d["page_table"], d["cu_q"], d["kv_len"], 8, 1e4)
+
+
+def test_calls_reach_the_library(launches):
+    attn()
+    append()
+    assert [c[0] for c in launches] == ["launch_attn_paged", "launch_rope_kv_append_paged"]
+
+
+@pytest.mark.parametrize("ws", [lambda: torch.empty(1 << 13, dtype=torch.uint8)[::2], lambda: torch.empty(64, 64, dtype=torch.uint8)[:, 0],
+                                lambda: torch.empty(1, dtype=torch.uint8).expand(1 << 20)])
+def test_a_workspace_must_be_contiguous(launches, ws):
+    """Its bytes are counted from the elements: those of a view with gaps are not all its own, an expanded one has only one."""
+    with pytest.raises(ValueError, match="scratch"):
+        attn(scratch=ws())
+    assert not launches
