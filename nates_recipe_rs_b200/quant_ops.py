@@ -402,6 +402,8 @@ def _paged(kpages, vpages, page_table, n_seqs):
     if page_table.dim() != 2 or page_table.shape[0] != n_seqs:
         raise ValueError(f"page_table: expected (n_seqs = {n_seqs}, pages)")
     width, page = page_table.shape[1], page_size * nkv * hd
+    if n_pages > 1 and (ks[0] < page or vs[0] < page):  # (a stride of 0 would mean back to back to the library)
+        raise ValueError("kpages and vpages: expected pages that do not share memory")
     return _lib.PagedKV(kpages.data_ptr(), vpages.data_ptr(), _DT[dtype], n_pages, page_size, nkv, hd, ks[0] if n_pages > 1 else page,
                         vs[0] if n_pages > 1 else page, _int32(page_table, n_seqs * width, index, "page_table"), width)
 

@@ -46,3 +46,13 @@ def test_a_workspace_must_be_contiguous(launches, ws):
     with pytest.raises(ValueError, match="scratch"):
         attn(scratch=ws())
     assert not launches
+
+
+@pytest.mark.parametrize("which", ["kpages", "vpages"])
+def test_pages_must_not_share_memory(launches, which):
+    """An expanded pool has a page stride of 0, which the library reads as 'back to back'; overlapping pages are no pool either."""
+    for pages in (torch.zeros(1, 16, 2, 64, dtype=F16).expand(6, 16, 2, 64), torch.zeros(1 << 14, dtype=F16).as_strided((6, 16, 2, 64), (1024, 128, 64, 1))):
+        for call in (attn, append):
+            with pytest.raises(ValueError, match="pages"):
+                call(**{which: pages})
+    assert not launches
