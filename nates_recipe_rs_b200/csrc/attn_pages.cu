@@ -93,10 +93,10 @@ int launch_rope_kv_append_paged(const void* qkv, int qkv_dtype, long qkv_stride,
     if (int st = check_pool(kv, p.k_page, p.v_page)) return st;
     if (qkv_dtype != QMM_DT_F32 && qkv_dtype != QMM_DT_F16 && qkv_dtype != QMM_DT_BF16) return QMM_ERR_TYPE;
     const int hd = kv->head_dim, nkv = kv->n_kv_heads;
-    if (n_q_heads <= 0 || rotary_dim < 0 || rotary_dim % 2 || rotary_dim > hd || qkv_stride < (long)(n_q_heads + 2 * nkv) * hd || !(theta > 0.f) ||
-        std::isinf(theta))
+    const long row = ((long)n_q_heads + 2l * nkv) * hd;
+    if (n_q_heads <= 0 || rotary_dim < 0 || rotary_dim % 2 || rotary_dim > hd || qkv_stride < row || !(theta > 0.f) || std::isinf(theta))
         return QMM_ERR_SHAPE;
-    if (rotary_dim > 2 * KVA_MAX_PAIRS || hd > 1024 || (long)(n_q_heads + 2 * nkv) * hd > 1 << 22) return QMM_ERR_UNSUPPORTED;
+    if (rotary_dim > 2 * KVA_MAX_PAIRS || hd > 1024 || row > 1 << 22) return QMM_ERR_UNSUPPORTED;
     const int size_in = qkv_dtype == QMM_DT_F32 ? 4 : 2;
     if (misaligned(qkv, size_in) || misaligned(q_out, 2)) return QMM_ERR_ALIGN;
     if (qkv == q_out) return QMM_ERR_SHAPE;
@@ -115,7 +115,7 @@ int launch_rope_kv_append_paged(const void* qkv, int qkv_dtype, long qkv_stride,
     // As few CTAs as run at once (six per SM), so that what a CTA does before its first byte (finding the sequences, the angles) is
     // not paid in two rounds: 2431 tokens of 20 heads of 96 take 7.6 us with three tokens per CTA, 11.2 with one; but no more work
     // than twice what its threads take at a time, or two tokens: 12122 tokens of 80 heads of 128 take 121 us with two, 131 with eight
-    const long units = (long)(n_q_heads + 2 * nkv) * hd / 16, at_once = 6l * sm_count();
+    const long units = row / 16, at_once = 6l * sm_count();
     const long most = std::min<long>(KVA_MAX_TOKENS, std::max<long>(2, 2 * KVA_THREADS / std::max<long>(units, 1)));
     p.tokens = (int)std::min(most, std::max<long>(1, (seqs->total_q + at_once - 1) / at_once));
     cudaStream_t s = as_stream(stream);
