@@ -333,10 +333,11 @@ int launch_attn_prefill_f16kv_at(const float* q, const void* k16, const void* v1
  * launch_attn_paged: row r of q (the pool's type) against the keys of its sequence at positions up to its own:
  *   out[r,h] = sum_t w_t v_t / sum_t w_t, w_t = exp(kq_scale * q_r.k_t - max), over t <= position, and t > position - window
  *   when window > 0.  A row that sees no key is 0.  out f16, bf16 or f32.  Query head h reads kv head h / (n_q_heads /
- *   n_kv_heads), at most 64 per kv head; head_dim 32, 64, 96, 128 or 256; page_size a multiple of 8; kq_scale positive and
- *   finite; q 16-byte aligned, q_stride a multiple of 8.  A key or value that a row does not see has no influence on it,
- *   whatever it holds (NaN and infinities too).  scratch: qmm_attn_paged_scratch_bytes(...) bytes of caller-owned device
- *   memory, 16-byte aligned, not shared with a call that may run at the same time; nothing in it needs clearing.
+ *   n_kv_heads), at most 64 per kv head; head_dim 32, 64, 96, 128 or 256; page_size a multiple of 8; kq_scale positive, at
+ *   most 2.3e38 (its product with log2(e) is an f32, as kq_scale * log2(e) * q_r.k_t has to be); q 16-byte aligned, q_stride a
+ *   multiple of 8.  A key or value that a row does not see has no influence on it, whatever it holds (NaN and infinities too).
+ *   scratch: qmm_attn_paged_scratch_bytes(...) bytes of caller-owned device memory, 16-byte aligned, not shared with a call that
+ *   may run at the same time; nothing in it needs clearing.
  * launch_attn_packed: the same without a cache, for whole prompts: the keys and values are rows of the batch (kv_len and max_kv
  *   unused; k and v in q's type, rows k_stride / v_stride elements apart, multiples of 8), so row i of a sequence sees rows 0..i
  *   of it.

@@ -62,7 +62,8 @@ static int check_out(const void* out, int dtype, long stride, int nqh, int hd) {
     if (misaligned(out, dtype == QMM_DT_F32 ? 8 : 4) || stride % 2) return QMM_ERR_ALIGN;
     return QMM_OK;
 }
-static bool bad_scale(float s) { return !(s > 0.f) || std::isinf(s); }
+constexpr float LOG2_E = 1.4426950408889634f;  // weights are computed as exp2(x log2(e))
+static bool bad_scale(float s) { return !(s > 0.f) || std::isinf(s * LOG2_E); }
 
 // Up to 16 (token, query head of the group) rows per sequence and kv head: decode, bound by the cache (attn_rows.cu); more rows:
 // the tcgen05 form (attn_tiles.cu), whose tiles of 128 rows would be mostly empty below that
@@ -151,7 +152,7 @@ int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, cons
     p.table_stride = kv->table_stride, p.page_size = kv->page_size, p.n_pages = kv->n_pages;
     p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = seqs->max_kv;
     p.nqh = n_q_heads, p.nkv = nkv, p.group = n_q_heads / nkv, p.window = window, p.out_dtype = out_dtype;
-    p.scale_log2 = kq_scale * 1.4426950408889634f;
+    p.scale_log2 = kq_scale * LOG2_E;
     // more rows whose items would not fill the GPU several times over: their tiles are shared evenly, as those of decode always are
     const bool narrow = attn_narrow(seqs->max_q, p.group);
     p.stream_k = ((long)p.total_q * p.group / attn_tiles_rows(hd) + 1) * nkv < 4l * sm_count();
@@ -178,7 +179,7 @@ int launch_attn_packed(const void* q, const void* k, const void* v, int dtype, l
     p.q_stride = q_stride, p.out_stride = out_stride, p.k_row = k_stride, p.v_row = v_stride;
     p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = seqs->max_q;
     p.nqh = n_q_heads, p.nkv = nkv, p.group = n_q_heads / nkv, p.window = window, p.out_dtype = out_dtype;
-    p.scale_log2 = kq_scale * 1.4426950408889634f;
+    p.scale_log2 = kq_scale * LOG2_E;
     p.k_page = (long)p.total_q * k_stride, p.v_page = (long)p.total_q * v_stride;  // one page of all rows
     return attn_run(false, p, dtype, hd, p.total_q, 1, as_stream(stream));
 }
