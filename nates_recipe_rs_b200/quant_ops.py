@@ -352,6 +352,7 @@ def gpu_gqa_attn_at_into(q, k16, v16, out, t, t_kv, q_pos0, nqh, nkv, hd, prefix
 
 
 # ---- a KV cache in pages, and batches of sequences of different lengths ------------------------
+# (a batch without rows or without sequences, whose tensors may have no address, is checked and nothing is launched)
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -423,6 +424,8 @@ def gpu_rope_kv_append_paged_into(qkv, q_out, kpages, vpages, page_table, cu_q, 
     if _row_stride(q_out, nqh * hd, "q_out", index, total) != nqh * hd:
         raise ValueError("q_out: expected a contiguous tensor")
     batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), _int32(kv_len, n_seqs, index, "kv_len"), n_seqs, total, total, 0x7FFFFFFF)
+    if total == 0 or n_seqs == 0:
+        return
     _launch_on(index, "launch_rope_kv_append_paged", qkv.data_ptr(), _DT[qkv.dtype], stride, q_out.data_ptr(), kv, batch, nqh,
                hd if rotary_dim is None else rotary_dim, theta)
 
@@ -448,11 +451,13 @@ def gpu_gqa_attn_paged_into(q, kpages, vpages, page_table, cu_q, kv_len, out, nq
     q_stride, o_stride = _row_stride(q, cols, "q", index), _row_stride(out, cols, "out", index, total)
     if q.dtype != kpages.dtype or out.dtype not in _DT:
         raise TypeError("q must have the cache's type, out be float32, float16 or bfloat16")
+    batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), _int32(kv_len, n_seqs, index, "kv_len"), n_seqs, total, max_q, max_kv)
+    if total == 0 or n_seqs == 0:
+        return
     if scratch is None:
         scratch = gpu_gqa_attn_paged_scratch(q, kpages, kv_len, nqh, max_q, max_kv)
     elif scratch.get_device() != index or not scratch.is_contiguous():  # (its bytes are counted from its elements)
         raise ValueError(f"scratch: expected a contiguous tensor on cuda:{index}")
-    batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), _int32(kv_len, n_seqs, index, "kv_len"), n_seqs, total, max_q, max_kv)
     _launch_on(index, "launch_attn_paged", q.data_ptr(), q_stride, kv, batch, out.data_ptr(), _DT[out.dtype], o_stride, scratch.data_ptr(),
                scratch.numel() * scratch.element_size(), nqh, window, kq_scale)
 
@@ -464,11 +469,15 @@ def gpu_gqa_attn_packed_into(q, k, v, cu_q, out, nqh, nkv, hd, max_q, kq_scale=1
     index, total, n_seqs, dtype = q.get_device(), q.shape[0], cu_q.numel() - 1, q.dtype
     if index < 0:
         raise ValueError("q: expected a CUDA tensor")
+    if n_seqs < 0:
+        raise ValueError("cu_q: expected one element more than there are sequences")
     q_stride, k_stride = _row_stride(q, nqh * hd, "q", index), _row_stride(k, nkv * hd, "k", index, total)
     v_stride, o_stride = _row_stride(v, nkv * hd, "v", index, total), _row_stride(out, nqh * hd, "out", index, total)
     if dtype not in (torch.float16, torch.bfloat16) or k.dtype != dtype or v.dtype != dtype or out.dtype not in _DT:
         raise TypeError("q, k and v must all be float16 or all bfloat16, out float32, float16 or bfloat16")
     batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), None, n_seqs, total, max_q, max_q)
+    if total == 0 or n_seqs == 0:
+        return
     _launch_on(index, "launch_attn_packed", q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[dtype], q_stride, k_stride, v_stride, batch, out.data_ptr(),
                _DT[out.dtype], o_stride, nqh, nkv, hd, window, kq_scale)
 

@@ -56,3 +56,24 @@ def test_pages_must_not_share_memory(launches, which):
             with pytest.raises(ValueError, match="pages"):
                 call(**{which: pages})
     assert not launches
+
+
+def packed(rows, cu):
+    x = torch.zeros(rows, 12 * 64, dtype=F16)
+    ops.gpu_gqa_attn_packed_into(x[:, :512], x[:, 512:640], x[:, 640:], cu, torch.zeros(rows, 512), 8, 2, 64, 0)
+
+
+@pytest.mark.parametrize("n_seqs,rows", [(2, 0), (0, 0), (0, 3)])
+def test_batches_without_rows_or_sequences_do_nothing(launches, n_seqs, rows):
+    """A server's step without new tokens: tensors of no elements have no address to hand to the library."""
+    kw = dict(q=torch.zeros(rows, 512, dtype=F16), cu_q=torch.zeros(n_seqs + 1, dtype=I32), kv_len=torch.zeros(n_seqs, dtype=I32),
+              page_table=torch.zeros(n_seqs, 3, dtype=I32))
+    attn(out=torch.zeros(rows, 512), **kw)
+    append(qkv=torch.zeros(rows, 768), out=torch.zeros(rows, 512, dtype=F16), **kw)
+    packed(rows, kw["cu_q"])
+    assert not launches
+    for kw in (dict(kw, page_table=kw["page_table"].long()), dict(kw, cu_q=kw["cu_q"].float()), dict(kw, q=kw["q"][:, :-1])):
+        with pytest.raises(ValueError):
+            attn(out=torch.zeros(rows, 512), **kw)
+    with pytest.raises(ValueError, match="cu_q"):
+        packed(rows, torch.zeros(0, dtype=I32))
