@@ -391,6 +391,7 @@ def _int32(t, n, index, name):
 
 
 def _paged(kpages, vpages, page_table, n_seqs):
+    """The pool, and the longest sequence that the page table has room for (its rows may be part of longer ones)."""
     shape, dtype, index = kpages.shape, kpages.dtype, kpages.get_device()
     if len(shape) != 4 or vpages.shape != shape:
         raise ValueError("kpages and vpages: expected two tensors (n_pages, page_size, n_kv_heads, head_dim)")
@@ -405,25 +406,29 @@ def _paged(kpages, vpages, page_table, n_seqs):
     width, page = page_table.shape[1], page_size * nkv * hd
     if n_pages > 1 and (ks[0] < page or vs[0] < page):  # (a stride of 0 would mean back to back to the library)
         raise ValueError("kpages and vpages: expected pages that do not share memory")
+    ts = page_table.stride()
+    t_stride = ts[0] if n_seqs > 1 else width
+    if page_table.dtype != torch.int32 or page_table.get_device() != index or (width > 1 and ts[1] != 1) or t_stride < width:
+        raise ValueError(f"page_table: expected an int32 tensor on cuda:{index}, rows contiguous and apart")
     return _lib.PagedKV(kpages.data_ptr(), vpages.data_ptr(), _DT[dtype], n_pages, page_size, nkv, hd, ks[0] if n_pages > 1 else page,
-                        vs[0] if n_pages > 1 else page, _int32(page_table, n_seqs * width, index, "page_table"), width)
+                        vs[0] if n_pages > 1 else page, page_table.data_ptr(), t_stride), min(width * page_size, 0x7FFFFFFF)
 
 
 def gpu_rope_kv_append_paged_into(qkv, q_out, kpages, vpages, page_table, cu_q, kv_len, nqh, theta, rotary_dim=None):
     """New tokens of a batch of sequences into a paged cache (launch_rope_kv_append_paged of include/qmm.h): the q and k heads
     of qkv (rows, (nqh + 2 nkv) * hd; f32, f16 or bf16; rows may be strided) rotated at their positions, q to q_out (rows,
     nqh * hd), k and v to their slots of kpages / vpages (n_pages, page_size, nkv, hd).  The tokens of sequence s are rows
-    cu_q[s] .. cu_q[s+1]-1 and its last positions, kv_len[s] its length with them; page_table (n_seqs, pages) int32.
-    rotary_dim None: the whole head."""
+    cu_q[s] .. cu_q[s+1]-1 and its last positions, kv_len[s] its length with them; page_table (n_seqs, pages) int32, whose rows
+    may be parts of longer ones.  rotary_dim None: the whole head."""
     index, n_seqs, total = kpages.get_device(), kv_len.numel(), qkv.shape[0]
-    kv = _paged(kpages, vpages, page_table, n_seqs)
+    kv, room = _paged(kpages, vpages, page_table, n_seqs)
     hd = kv.head_dim
     stride = _row_stride(qkv, (nqh + 2 * kv.n_kv_heads) * hd, "qkv", index)
     if q_out.dtype != kpages.dtype or qkv.dtype not in _DT:
         raise TypeError("q_out must have the cache's type, qkv be float32, float16 or bfloat16")
     if _row_stride(q_out, nqh * hd, "q_out", index, total) != nqh * hd:
         raise ValueError("q_out: expected a contiguous tensor")
-    batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), _int32(kv_len, n_seqs, index, "kv_len"), n_seqs, total, total, 0x7FFFFFFF)
+    batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), _int32(kv_len, n_seqs, index, "kv_len"), n_seqs, total, total, room)
     if total == 0 or n_seqs == 0:
         return
     _launch_on(index, "launch_rope_kv_append_paged", qkv.data_ptr(), _DT[qkv.dtype], stride, q_out.data_ptr(), kv, batch, nqh,
@@ -446,12 +451,12 @@ def gpu_gqa_attn_paged_into(q, kpages, vpages, page_table, cu_q, kv_len, out, nq
     bf16 (rows of either may be strided); a row sees the positions up to its own, the last `window` of them if window > 0, and
     is 0 when it sees none.  max_q, max_kv: at least the most new tokens and the longest sequence of the batch."""
     index, n_seqs, total = kpages.get_device(), kv_len.numel(), q.shape[0]
-    kv = _paged(kpages, vpages, page_table, n_seqs)
+    kv, room = _paged(kpages, vpages, page_table, n_seqs)
     cols = nqh * kv.head_dim
     q_stride, o_stride = _row_stride(q, cols, "q", index), _row_stride(out, cols, "out", index, total)
     if q.dtype != kpages.dtype or out.dtype not in _DT:
         raise TypeError("q must have the cache's type, out be float32, float16 or bfloat16")
-    batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), _int32(kv_len, n_seqs, index, "kv_len"), n_seqs, total, max_q, max_kv)
+    batch = _lib.SeqBatch(_int32(cu_q, n_seqs + 1, index, "cu_q"), _int32(kv_len, n_seqs, index, "kv_len"), n_seqs, total, max_q, min(max_kv, room))
     if total == 0 or n_seqs == 0:
         return
     if scratch is None:

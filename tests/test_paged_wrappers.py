@@ -77,3 +77,26 @@ def test_batches_without_rows_or_sequences_do_nothing(launches, n_seqs, rows):
             attn(out=torch.zeros(rows, 512), **kw)
     with pytest.raises(ValueError, match="cu_q"):
         packed(rows, torch.zeros(0, dtype=I32))
+
+
+def test_page_tables_inside_wider_ones(launches):
+    """A server's table cut to the pages in use: its rows lie further apart than they are long, and no length reaches past the cut."""
+    wide = torch.zeros(5, 40, dtype=I32)
+    table = wide[1:3, 4:7]
+    attn(page_table=table)
+    attn(page_table=table, max_kv=1000)
+    append(page_table=table)
+    attn(page_table=wide[1:2, 4:7], q=torch.zeros(3, 512, dtype=F16), cu_q=torch.zeros(2, dtype=I32), kv_len=torch.zeros(1, dtype=I32))
+    (_, a), (_, long), (_, b), (_, one) = launches
+    for pool, batch in ((a[2], a[3]), (long[2], long[3]), (b[4], b[5])):
+        assert pool.page_table == table.data_ptr() and pool.table_stride == 40 and batch.n_seqs == 2
+    assert (a[3].max_kv, long[3].max_kv, b[5].max_kv, one[3].max_kv) == (30, 48, 48, 30)
+
+
+@pytest.mark.parametrize("table", [lambda: torch.zeros(2, 6, dtype=I32)[:, ::2], lambda: torch.zeros(3, 2, dtype=I32).T, lambda: torch.zeros(1, 3, dtype=I32).expand(2, 3),
+                                   lambda: torch.zeros(2, 3), lambda: torch.zeros(3, 3, dtype=I32), lambda: torch.zeros(6, dtype=I32)])
+def test_page_tables_that_are_refused(launches, table):
+    for call in (attn, append):
+        with pytest.raises(ValueError, match="page_table"):
+            call(page_table=table())
+    assert not launches
