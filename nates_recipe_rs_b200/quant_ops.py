@@ -399,7 +399,10 @@ def _paged(kpages, vpages, page_table, n_seqs):
         raise TypeError("kpages and vpages must both be float16 or both bfloat16")
     n_pages, page_size, nkv, hd = shape
     ks, vs = kpages.stride(), vpages.stride()
-    if ks[1:] != (nkv * hd, hd, 1) or vs[1:] != ks[1:] or index < 0 or vpages.get_device() != index:
+    want = (nkv * hd, hd, 1)
+    if (ks[1:] != want or vs[1:] != want) and any(n > 1 and st != w for d in (ks, vs) for n, st, w in zip(shape[1:], d[1:], want)):
+        raise ValueError("kpages and vpages: expected CUDA tensors with contiguous pages, on one device")
+    if index < 0 or vpages.get_device() != index:
         raise ValueError("kpages and vpages: expected CUDA tensors with contiguous pages, on one device")
     if page_table.dim() != 2 or page_table.shape[0] != n_seqs:
         raise ValueError(f"page_table: expected (n_seqs = {n_seqs}, pages)")

@@ -100,3 +100,21 @@ def test_page_tables_that_are_refused(launches, table):
         with pytest.raises(ValueError, match="page_table"):
             call(page_table=table())
     assert not launches
+
+
+@pytest.mark.parametrize("pool", [lambda: torch.zeros(6, 1, 16, 64, dtype=F16).transpose(1, 2), lambda: torch.zeros(6, 1, 64, dtype=F16).as_strided((6, 1, 1, 64), (64, 7, 9, 1)),
+                                  lambda: torch.zeros(6, 2, 1, 64, dtype=F16).as_strided((6, 1, 2, 64), (128, 999, 64, 1))])
+def test_strides_of_dimensions_of_one_element_do_not_matter(launches, pool):
+    """One kv head kept heads first, or one slot a page: the pages are contiguous whatever such a dimension's stride says."""
+    k, v = pool(), pool()
+    page, nkv = k.shape[1:3]
+    kw = dict(kpages=k, vpages=v, qkv=torch.zeros(3, (8 + 2 * nkv) * 64))
+    attn(**kw)
+    append(**kw)
+    for _, args in launches:
+        pool_arg = next(a for a in args if hasattr(a, "k_page_stride"))
+        assert (pool_arg.page_size, pool_arg.n_kv_heads, pool_arg.k_page_stride) == (page, nkv, page * nkv * 64)
+    assert len(launches) == 2
+    for bad in (torch.zeros(6, 2, 16, 64, dtype=F16).transpose(1, 2), torch.zeros(6, 16, 1, 128, dtype=F16)[..., ::2]):
+        with pytest.raises(ValueError, match="pages"):
+            attn(kpages=bad, vpages=bad)
