@@ -108,9 +108,8 @@ def test_strides_of_dimensions_of_one_element_do_not_matter(launches, pool):
     """One kv head kept heads first, or one slot a page: the pages are contiguous whatever such a dimension's stride says."""
     k, v = pool(), pool()
     page, nkv = k.shape[1:3]
-    kw = dict(kpages=k, vpages=v, qkv=torch.zeros(3, (8 + 2 * nkv) * 64))
-    attn(**kw)
-    append(**kw)
+    attn(kpages=k, vpages=v)
+    append(kpages=k, vpages=v, qkv=torch.zeros(3, (8 + 2 * nkv) * 64))
     for _, args in launches:
         pool_arg = next(a for a in args if hasattr(a, "k_page_stride"))
         assert (pool_arg.page_size, pool_arg.n_kv_heads, pool_arg.k_page_stride) == (page, nkv, page * nkv * 64)
