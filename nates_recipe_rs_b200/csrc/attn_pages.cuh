@@ -81,12 +81,14 @@ __device__ __noinline__ SeqInfo seq_info(const AttnParams& p, int s) {
 struct KeyRange {
     int a, b, a2, b2;
 };
+// The first key that position pos sees (a position before 0 sees none: kept out of the difference, which a wide window would overflow)
+__device__ __forceinline__ int first_key(const AttnParams& p, int pos) { return p.window ? max(max(pos, 0) - p.window + 1, 0) : 0; }
 __device__ __forceinline__ KeyRange key_range(const AttnParams& p, const SeqInfo& si, int tok0, int tok1) {
     const int p0 = si.kv - si.q_len + tok0, p1 = si.kv - si.q_len + tok1 - 1;  // first and last position
     KeyRange r;
-    r.a = p.window ? max(0, p0 - p.window + 1) : 0;
+    r.a = first_key(p, p0);
     r.b = max(p1 + 1, 0);
-    r.a2 = p.window ? max(0, p1 - p.window + 1) : 0;
+    r.a2 = first_key(p, p1);
     r.b2 = max(p0 + 1, 0);
     return r;
 }

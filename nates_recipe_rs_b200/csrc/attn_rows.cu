@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(AR_THREADS, ArShape<HD>::CTAS_PER_SM) attn_row
             const int r = qr + 8 * e;
             const int pos = pos0 + (r0 + r) / p.group;
             hi[e] = r < n_rows ? max(pos + 1, 0) : 0;
-            lo[e] = p.window ? max(0, pos - p.window + 1) : 0;
+            lo[e] = first_key(p, pos);
         }
         uint32_t qf[Sh::Q_REGS ? HD / 16 : 1][4];
         const uint32_t qa = smem_u32(qs + (lane & 15) * QPITCH + (lane >> 4) * 8);

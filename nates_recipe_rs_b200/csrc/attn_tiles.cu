@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
             for (int e = 0; e < 2; ++e) {
                 const int tok = w.tok0 + wg * tpt + ((row0 + 8 * e) * p.group_inv >> 16), pos = pos0 + tok;
                 hi[e] = row0 + 8 * e < tile_rows && tok < w.tok1 ? max(pos + 1, 0) : 0;
-                lo[e] = p.window ? max(0, pos - p.window + 1) : 0;
+                lo[e] = first_key(p, pos);
             }
             float m[2] = {-INFINITY, -INFINITY};
             uint64_t l2[2] = {0ull, 0ull};  // sums of this lane's even and odd columns
