@@ -715,8 +715,10 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                 for (int e = 0; e < 2; ++e) {
                     mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 1));
                     mt[e] = fmaxf(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 2));
-                    // (rows that are none, hi 0, hold anything: they have no say, or reruns would not be bit identical)
-                    grew |= hi[e] > 0 && ((mt[e] - m[e]) * c > 8.f || (m[e] == -INFINITY && mt[e] > -INFINITY));
+                    // A row's maximum moves by what the row itself has seen, not when another row of the warp makes it rescale: the
+                    // roundings of P depend on it.  (Rows that are none, hi 0, hold anything: reruns would not be bit identical)
+                    if (t == t0 || (hi[e] > 0 && ((mt[e] - m[e]) * c > 8.f || (m[e] == -INFINITY && mt[e] > -INFINITY)))) grew = true;
+                    else mt[e] = m[e];
                 }
                 bool o_done = !Sh::WIDE || t == t0;  // the outputs so far are complete (two row tiles: they are when the scores are)
                 if (t == t0) {
@@ -733,9 +735,8 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                     float f[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float mn = fmaxf(m[e], mt[e]);
-                        f[e] = mn == -INFINITY ? 1.f : fast_exp2((m[e] - mn) * c);
-                        m[e] = mn, l2[e] = mul2(l2[e], f32x2(f[e], f[e]));
+                        f[e] = mt[e] == m[e] ? 1.f : fast_exp2((m[e] - mt[e]) * c);
+                        m[e] = mt[e], l2[e] = mul2(l2[e], f32x2(f[e], f[e]));
                     }
 #pragma unroll 1
                     for (int q = 0; q < HD / 32; ++q) {
