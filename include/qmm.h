@@ -335,7 +335,8 @@ int launch_attn_prefill_f16kv_at(const float* q, const void* k16, const void* v1
  *   when window > 0.  A row that sees no key is 0.  out f16, bf16 or f32.  Query head h reads kv head h / (n_q_heads /
  *   n_kv_heads), at most 64 per kv head; head_dim 32, 64, 96, 128 or 256; page_size a multiple of 8; kq_scale positive, at
  *   most 2.3e38 (its product with log2(e) is an f32, as kq_scale * log2(e) * q_r.k_t has to be); q 16-byte aligned, q_stride a
- *   multiple of 8.  A key or value that a row does not see has no influence on it, whatever it holds (NaN and infinities too).
+ *   multiple of 8; sequences of up to 2^31 - 4096 tokens (longer ones are cut to that, status 7).  A key or value that a row
+ *   does not see has no influence on it, whatever it holds (NaN and infinities too).
  *   scratch: qmm_attn_paged_scratch_bytes(...) bytes of caller-owned device memory, 16-byte aligned, not shared with a call that
  *   may run at the same time; nothing in it needs clearing.
  * launch_attn_packed: the same without a cache, for whole prompts: the keys and values are rows of the batch (kv_len and max_kv

@@ -150,7 +150,7 @@ int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, cons
     p.table = kv->page_table, p.cu_q = seqs->cu_q, p.kv_len = seqs->kv_len, p.scratch = static_cast<float*>(scratch);
     p.q_stride = q_stride, p.out_stride = out_stride, p.k_row = p.v_row = (long)nkv * hd;
     p.table_stride = kv->table_stride, p.page_size = kv->page_size, p.n_pages = kv->n_pages;
-    p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = seqs->max_kv;
+    p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = std::min(seqs->max_kv, ATT_MAX_KEYS);
     p.nqh = n_q_heads, p.nkv = nkv, p.group = n_q_heads / nkv, p.window = window, p.out_dtype = out_dtype;
     p.scale_log2 = kq_scale * LOG2_E;
     // more rows whose items would not fill the GPU several times over: their tiles are shared evenly, as those of decode always are

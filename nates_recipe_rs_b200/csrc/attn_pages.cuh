@@ -13,6 +13,7 @@ namespace qmm {
 
 constexpr int ATT_MAX_GROUP = 64;   // query heads of one kv head
 constexpr int ATT_MAX_SEQS = 1 << 20;
+constexpr int ATT_MAX_KEYS = 0x7FFFFFFF - 4095;  // positions of a tile past the last key, and of its up to 32 boxes, stay in 32 bits
 
 struct AttnParams {
     const void* q;

@@ -19,6 +19,28 @@ def test_windows_longer_than_any_sequence(ops, hd, q_len, kv, window):
     assert torch.equal(check(ops, b, window=window), check(ops, b))
 
 
+# ---- lengths ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("q_len", [1, 20])
+def test_the_longest_sequences(ops, q_len):
+    """2^31 - 4096 keys, every page of the table the same one, all scores 0 and all values 1: sums of ones below 2^24 are exact and
+    those of the parts are rounded alike above and below the line, so the outputs are 1.  Longer ones are cut and reported."""
+    page, longest = 1 << 16, (1 << 31) - 4096
+    k = torch.zeros(1, page, 1, 32, dtype=F16, device="cuda")
+    v = torch.ones_like(k)
+    table = torch.zeros(1, 1 << 15, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, q_len], dtype=torch.int32, device="cuda")
+    q = torch.ones(q_len, 32, dtype=F16, device="cuda")
+    for kv in (longest, longest + 1, (1 << 31) - 1):
+        out = torch.full((q_len, 32), 77.0, dtype=F16, device="cuda")
+        ops.gpu_gqa_attn_paged_into(q, k, v, table, cu, torch.tensor([kv], dtype=torch.int32, device="cuda"), out, 1, q_len, kv)
+        if kv == longest:
+            ops.check_launch()
+            assert (out == 1).all()
+        else:
+            with pytest.raises(RuntimeError, match="status 7"):
+                ops.check_launch()
+
+
 # ---- what a row does not see -----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("hd,nqh,nkv", [(128, 8, 2), (64, 7, 1), (256, 4, 4), (32, 12, 4)])
 def test_a_large_later_key_changes_no_bit_of_the_rows_before(ops, hd, nqh, nkv):
