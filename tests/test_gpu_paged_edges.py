@@ -65,3 +65,121 @@ def test_a_large_later_row_of_a_packed_prompt_changes_no_bit_of_the_rows_before(
     ops.check_launch()
     assert not torch.equal(one[290:300], two[290:300])
     assert torch.equal(one[:290], two[:290]) and torch.equal(one[300:], two[300:])
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf")])
+@pytest.mark.parametrize("hd,q_len", [(128, 1), (64, 2), (256, 3), (128, 100), (64, 300), (256, 80), (32, 70)])
+def test_infinite_keys(ops, hd, q_len, bad):
+    """Rows before it do not see it; a row that sees it is NaN where its score is +inf, and what it is without that key where its
+    score is -inf."""
+    kv = q_len + 77
+    b = ref.Batch([q_len, 5], [kv, 9], 8, 2, hd, 16, BF16, seed=q_len + hd)
+    b.q.view(-1, 8, hd)[:, 4:, 0] = torch.tensor([0.5, -0.5, 1.5, -2.0], device="cuda")  # heads of both signs
+    want, tol = ref.expect(b, hd ** -0.5, 0, BF16)
+    key = kv - max(q_len // 3, 1)
+    page, slot = int(b.table[0, key // 16]), key % 16
+    b.k[page, slot, 1, 0] = bad
+    n = kv - key  # tokens that see it: the last ones
+    rows = slice(q_len - n, q_len)
+    keep = [t for t in range(kv) if t != key]
+    want[rows], tol[rows] = (torch.cat([whole, gone[:, 4:]], dim=1) for whole, gone in zip(
+        (want[rows][:, :4], tol[rows][:, :4]),
+        ref.attention(b.q[rows].view(n, 8, hd), b.keys[0][keep], b.vals[0][keep], hd ** -0.5, 0, BF16, BF16)))
+    got = paged(ops, b).view(-1, 8, hd)
+    ops.check_launch()
+    up = torch.zeros(b.total, 8, dtype=torch.bool, device="cuda")
+    up[rows, 4:] = b.q.view(-1, 8, hd)[rows][:, 4:, 0] * bad > 0
+    assert torch.isnan(got[up]).all()
+    ref.near(torch.where(up[..., None], 0.0, got.double()), torch.where(up[..., None], 0.0, want), torch.where(up[..., None], 0.0, tol))
+
+
+def test_values_near_the_end_of_a_bf16_cache(ops):
+    """Sums of values of 1e30 with probabilities of up to 256 (scores that grow slowly from key to key) stay finite."""
+    b = ref.Batch([1, 100], [900, 900], 8, 2, 64, 16, BF16, seed=31, values=1e30)
+    ramp = torch.linspace(0, 30, 900).to(BF16).cuda()
+    b.q.zero_()
+    b.q.view(-1, 8, 64)[..., 0] = 1.0
+    for s in range(2):
+        b.keys[s][:] = 0
+        b.keys[s][..., 0] = ramp[:, None]
+        for t in range(900):
+            b.k[int(b.table[s, t // 16]), t % 16] = b.keys[s][t]
+    check(ops, b, scale=1.0)
+
+
+# ---- long batches ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,nqh,nkv,q_lens,kv_lens", [
+    (128, 8, 2, [1500], [1500]), (64, 14, 2, [1100, 3], [1100, 4000]), (256, 4, 2, [700], [700]), (96, 12, 4, [900], [2500]),
+    (128, 16, 8, [30] * 60 + [1200], [300] * 60 + [1500]), (64, 16, 16, [17] * 150 + [600], [17] * 150 + [900]),
+    (256, 8, 8, [40] * 50 + [500], [40] * 50 + [500]), (128, 32, 1, [1] * 40 + [1], [200] * 40 + [9000])])
+def test_prompts_through_the_cache_and_batches_that_end_in_their_longest(ops, dtype, hd, nqh, nkv, q_lens, kv_lens):
+    check(ops, ref.Batch(q_lens, kv_lens, nqh, nkv, hd, 32, dtype, seed=hd + len(q_lens), spare_rows=1))
+
+
+@pytest.mark.parametrize("hd,nqh,nkv", [(128, 32, 8), (64, 4, 4), (256, 8, 4)])
+def test_packed_batches_that_end_in_their_longest(ops, hd, nqh, nkv):
+    lens = [30 + i % 50 for i in range(60)] + [1500]
+    qkv = torch.randn(sum(lens), (nqh + 2 * nkv) * hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(hd)).half()
+    b = pack(qkv, lens, nqh, nkv, hd, F16)
+    out = packed(ops, b, qkv)
+    ops.check_launch()
+    ref.near(out, *ref.expect(b, hd ** -0.5, 0, F16))
+
+
+# ---- tables and pages ------------------------------------------------------------------------------------------------
+def test_page_tables_inside_wider_ones(ops):
+    for q_lens, kv_lens in (([1, 1, 1], [100, 333, 7]), ([90, 7, 0], [100, 333, 20])):
+        b = ref.Batch(q_lens, kv_lens, 8, 2, 64, 16, F16, seed=41)
+        want = paged(ops, b)
+        n = b.table.shape[1]
+        wide = torch.full((3, n + 9), -5, dtype=torch.int32, device="cuda")
+        wide[:, 4:4 + n] = b.table
+        b.table = wide[:, 4:4 + n]
+        assert torch.equal(check(ops, b), want)
+        new = torch.randn(b.total, 12 * 64, device="cuda")
+        k, v, q_out = b.k.clone(), b.v.clone(), [torch.empty(b.total, 512, dtype=F16, device="cuda") for _ in range(2)]
+        ops.gpu_rope_kv_append_paged_into(new, q_out[0], b.k, b.v, b.table, b.cu, b.kv_len, 8, 1e4)
+        ops.gpu_rope_kv_append_paged_into(new, q_out[1], k, v, b.table.contiguous(), b.cu, b.kv_len, 8, 1e4)
+        ops.check_launch()
+        for x, y in ((b.k, k), (b.v, v), q_out):
+            assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+        b.max_kv = 16 * (n + 9)
+        b.kv_len[1] = 16 * n + 1  # one more than the columns given have room for
+        paged(ops, b)
+        with pytest.raises(RuntimeError, match="status 7"):
+            ops.check_launch()
+
+
+def test_a_bad_page_takes_nothing(ops):
+    """A new token whose table entry is no page of the pool is written nowhere: only the other sequence's pages change."""
+    for bad in (-1, 1 << 30, -(1 << 31)):
+        b = ref.Batch([1, 30], [50, 90], 8, 2, 128, 16, F16, seed=15, poison=False)
+        own = set(b.table[1, :6].tolist())
+        b.table[0, 3] = bad
+        k, v = b.k.clone(), b.v.clone()
+        ops.gpu_rope_kv_append_paged_into(torch.randn(31, 12 * 128, device="cuda"), torch.empty_like(b.q), b.k, b.v, b.table, b.cu, b.kv_len, 8, 1e4)
+        with pytest.raises(RuntimeError, match="status 6"):
+            ops.check_launch()
+        for x, y in ((b.k, k), (b.v, v)):
+            touched = set((x != y).flatten(1).any(dim=1).nonzero().flatten().tolist())
+            assert touched and touched <= own
+        assert len(own) < b.n_pages
+
+
+def test_batches_without_rows_do_nothing(ops):
+    k = torch.zeros(4, 16, 2, 64, dtype=F16, device="cuda")
+    cu, kv, table = (torch.zeros(*n, dtype=torch.int32, device="cuda") for n in ((3,), (2,), (2, 2)))
+    q = torch.empty(0, 512, dtype=F16, device="cuda")
+    ops.gpu_rope_kv_append_paged_into(torch.empty(0, 768, device="cuda"), q, k, k, table, cu, kv, 8, 1e4)
+    ops.gpu_gqa_attn_paged_into(q, k, k, table, cu, kv, torch.empty_like(q), 8, 0, 0)
+    ops.gpu_gqa_attn_packed_into(q, q[:, :128], q[:, :128], cu, torch.empty_like(q), 8, 2, 64, 0)
+    ops.check_launch()
+
+
+@pytest.mark.parametrize("ws", [lambda n: torch.empty(2 * n, dtype=torch.uint8, device="cuda")[::2], lambda n: torch.empty(1, dtype=torch.uint8, device="cuda").expand(n)])
+def test_workspaces_that_are_not_contiguous_are_refused(ops, ws):
+    b = ref.Batch([1, 2], [9, 30], 8, 2, 64, 16, F16, seed=23, poison=False)
+    n = ops.gpu_gqa_attn_paged_scratch(b.q, b.k, b.kv_len, 8, 2, 30).numel()
+    with pytest.raises(ValueError, match="scratch"):
+        paged(ops, b, scratch=ws(n))
