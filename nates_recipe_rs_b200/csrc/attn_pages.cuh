@@ -144,31 +144,6 @@ __device__ __noinline__ int find_item(const AttnParams& p, long target, long& be
     return found;
 }
 
-// As find_item, by one warp: 32 sequences at a time
-template <typename F>
-__device__ __noinline__ int warp_find_item(const AttnParams& p, long target, long& before) {
-    const int lane = threadIdx.x & 31;
-    before = 0;
-#pragma unroll 1
-    for (int base = 0; base < p.n_seqs; base += 32) {
-        const long long cnt = base + lane < p.n_seqs ? (long long)F::count(p, base + lane) : 0ll;
-        long long inc = cnt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, before + inc > target);
-        if (past) {
-            const int f = __ffs(past) - 1;
-            before += __shfl_sync(0xffffffffu, inc - cnt, f);
-            return base + f;
-        }
-        before += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    return -1;
-}
-
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
