@@ -439,8 +439,9 @@ def gpu_rope_kv_append_paged_into(qkv, q_out, kpages, vpages, page_table, cu_q, 
 
 
 def gpu_gqa_attn_paged_scratch(q, kpages, kv_len, nqh, max_q, max_kv):
-    """The workspace of gpu_gqa_attn_paged_into for these sizes (its contents need no clearing).  Calls that may run at the
-    same time need one each."""
+    """The workspace of gpu_gqa_attn_paged_into (its contents need no clearing).  Its size depends on the heads, on head_dim and on
+    whether max_q makes the call a decode step, not on the lengths (kv_len and max_kv are not looked at); one made for a larger
+    max_q serves smaller ones too.  Calls that may run at the same time need one each."""
     nkv, hd = kpages.shape[2], kpages.shape[3]
     with torch.cuda.device(q.device):
         n = lib().qmm_attn_paged_scratch_bytes(max_q, nqh, nkv, hd)
