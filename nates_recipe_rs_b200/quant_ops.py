@@ -468,7 +468,7 @@ def gpu_gqa_attn_paged_into(q, kpages, vpages, page_table, cu_q, kv_len, out, nq
     elif scratch.get_device() != index or not scratch.is_contiguous():  # (its bytes are counted from its elements)
         raise ValueError(f"scratch: expected a contiguous tensor on cuda:{index}")
     _launch_on(index, "launch_attn_paged", q.data_ptr(), q_stride, kv, batch, out.data_ptr(), _DT[out.dtype], o_stride, scratch.data_ptr(),
-               scratch.numel() * scratch.element_size(), nqh, window, kq_scale)
+               scratch.numel() * scratch.element_size(), nqh, min(window, 0x7FFFFFFF), kq_scale)
 
 
 def gpu_gqa_attn_packed_into(q, k, v, cu_q, out, nqh, nkv, hd, max_q, kq_scale=1.0, window=0):
@@ -488,7 +488,7 @@ def gpu_gqa_attn_packed_into(q, k, v, cu_q, out, nqh, nkv, hd, max_q, kq_scale=1
     if total == 0 or n_seqs == 0:
         return
     _launch_on(index, "launch_attn_packed", q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[dtype], q_stride, k_stride, v_stride, batch, out.data_ptr(),
-               _DT[out.dtype], o_stride, nqh, nkv, hd, window, kq_scale)
+               _DT[out.dtype], o_stride, nqh, nkv, hd, min(window, 0x7FFFFFFF), kq_scale)
 
 
 # ---- quantized dense layer ---------------------------------------------------------------

@@ -117,3 +117,12 @@ def test_strides_of_dimensions_of_one_element_do_not_matter(launches, pool):
     for bad in (torch.zeros(6, 2, 16, 64, dtype=F16).transpose(1, 2), torch.zeros(6, 16, 1, 128, dtype=F16)[..., ::2]):
         with pytest.raises(ValueError, match="pages"):
             attn(kpages=bad, vpages=bad)
+
+
+@pytest.mark.parametrize("window,given", [(0, 0), (7, 7), ((1 << 31) - 1, (1 << 31) - 1), (1 << 31, (1 << 31) - 1), ((1 << 32) + 5, (1 << 31) - 1), ((1 << 63) - 1, (1 << 31) - 1)])
+def test_windows_past_32_bits_hide_nothing(launches, window, given):
+    """The library takes 32 bits, and a number beyond them is not refused on the way there but loses its upper ones."""
+    attn(window=window)
+    x = torch.zeros(3, 768, dtype=F16)
+    ops.gpu_gqa_attn_packed_into(x[:, :512], x[:, 512:640], x[:, 640:], torch.zeros(2, dtype=I32), torch.zeros(3, 512), 8, 2, 64, 3, window=window)
+    assert [args[-2] for _, args in launches] == [given, given]
