@@ -171,15 +171,17 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ float lo2(uint64_t a) { return __uint_as_float((uint32_t)a); }
 __device__ __forceinline__ float hi2(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
-// P = exp2(s c - mc) of 64 keys to 32 columns of tensor memory; adds this lane's columns to l (before they are rounded)
+// P = exp2((s - m) c) of 64 keys to 32 columns of tensor memory; adds this lane's columns to l (before they are rounded).  The
+// difference comes first: in s c - m c, one instruction instead of two, the rounding of m c put P off by up to 2^(|m c| 2^-24), a
+// factor that changed when m moved and made P overflow from |m c| = 2^28 on; the times were the same (8192 tokens within 0.5 %)
 template <typename T>
-__device__ __forceinline__ void exp64(const uint32_t (&s)[32], float c, const float (&mc)[2], uint32_t tp, uint64_t (&l)[2]) {
+__device__ __forceinline__ void exp64(const uint32_t (&s)[32], float c, const float (&mu)[2], uint32_t tp, uint64_t (&l)[2]) {
     const uint64_t c2 = f32x2(c, c);
     uint32_t pk[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const int e = j & 1;
-        const uint64_t x = fma2(f32x2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), c2, f32x2(-mc[e], -mc[e]));
+        const uint64_t x = mul2(add2(f32x2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), f32x2(-mu[e], -mu[e])), c2);
         const uint64_t y = f32x2(fast_exp2(lo2(x)), fast_exp2(hi2(x)));
         l[e] = add2(l[e], y);
         pk[j] = pack2<T>(lo2(y), hi2(y));
@@ -758,7 +760,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                     }
                     ++n_turn;
                 }
-                const float mc[2] = {m[0] == -INFINITY ? 0.f : m[0] * c, m[1] == -INFINITY ? 0.f : m[1] * c};
+                const float mu[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll 1
                 for (int h = 1; h >= 0; --h) {  // the second half, in registers, first
                     if (h == 0) {
@@ -766,7 +768,7 @@ __global__ void __launch_bounds__(AtShape<HD>::THREADS, 1) attn_tiles_kernel(con
                         if (right) mask_right(sr, t * AT_TILE, hi);
                         if (left) mask_left(sr, t * AT_TILE, lo);
                     }
-                    exp64<T>(sr, c, mc, ts + AT_COL_P + 32 * h, l2);
+                    exp64<T>(sr, c, mu, ts + AT_COL_P + 32 * h, l2);
                     if (h == 1 && !o_done) {  // once per tile, and before P is announced: the issuer is then past the P before
                         ok = wait(&hdr->o_full[0], n_o, DEV_TIMEOUT_MMA);
                         ++n_o;

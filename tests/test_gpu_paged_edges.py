@@ -107,6 +107,38 @@ def test_values_near_the_end_of_a_bf16_cache(ops):
     check(ops, b, scale=1.0)
 
 
+def one_hot_batch(q_lens, kv_lens, hd, base, step, nqh=8, nkv=2, order=1):
+    """Scores that f32 holds exactly: q = (base, step, 0 ..), key t = (base, +-t, 0 ..), so q . k = base^2 +- step t."""
+    b = ref.Batch(q_lens, kv_lens, nqh, nkv, hd, 16, F16, seed=hd)
+    b.q.zero_()
+    b.q.view(-1, nqh, hd)[..., 0], b.q.view(-1, nqh, hd)[..., 1] = base, step
+    for s, n in enumerate(kv_lens):
+        b.keys[s].zero_()
+        b.keys[s][..., 0], b.keys[s][..., 1] = base, order * torch.arange(n, device="cuda").half()[:, None]
+        for t in range(n):
+            b.k[int(b.table[s, t // 16]), t % 16] = b.keys[s][t]
+    return b
+
+
+@pytest.mark.parametrize("order", [1, -1])
+@pytest.mark.parametrize("hd,q_len", [(64, 1), (128, 60), (64, 200), (256, 40), (32, 70)])
+def test_scores_far_from_zero(ops, hd, q_len, order):
+    """2^30 and more, whose differences decide.  With a scale of 1 the best key has all the weight; with 2^-6 the scores are 2^24
+    +- 2 t, which f32 holds and the weights have to follow: exact scores leave the bound of the probabilities' rounding, of f32
+    sums (600 keys) and of the output's rounding."""
+    b = one_hot_batch([q_len, 3], [600, 50], hd, 32768.0, 128.0, order=order)
+    for scale in (1.0, 2.0 ** -6):
+        out = paged(ops, b, scale=scale, out_dtype=F32).view(-1, 8, hd)
+        ops.check_launch()
+        for s, (n, t) in enumerate(zip(b.q_lens, b.kv_lens)):
+            pos, key = torch.arange(t - n, t, device="cuda")[:, None], torch.arange(t, device="cuda")[None]
+            x = torch.where(key <= pos, scale * (2.0 ** 30 + order * 128.0 * key.double()), float("-inf"))
+            p = torch.softmax(x, dim=1)
+            v = b.vals[s].double().repeat_interleave(4, dim=1)
+            want, size = torch.einsum("nt,thd->nhd", p, v), torch.einsum("nt,thd->nhd", p, v.abs())
+            ref.near(out[b.rows(s)], want, size * (2.0 ** -11 + 2.0 ** -19 + 700 * 2.0 ** -23) + 2.0 ** -25 * t * v.abs().max(), f"scale {scale}")
+
+
 # ---- long batches ----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("hd,nqh,nkv,q_lens,kv_lens", [
