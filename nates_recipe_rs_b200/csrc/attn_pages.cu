@@ -66,7 +66,10 @@ constexpr float LOG2_E = 1.4426950408889634f;  // weights are computed as exp2(x
 static bool bad_scale(float s) { return !(s > 0.f) || std::isinf(s * LOG2_E); }
 
 // Up to 16 (token, query head of the group) rows per sequence and kv head: decode, bound by the cache (attn_rows.cu); more rows:
-// the tcgen05 form (attn_tiles.cu), whose tiles of 128 rows would be mostly empty below that
+// the tcgen05 form (attn_tiles.cu), whose tiles of 128 rows are mostly empty below that.  Measured, us in attn_rows / attn_tiles,
+// 64 sequences of 1000 to 7300 tokens, f16: 32/8 heads of 128, 1 token (4 rows) 178 / 227, 4 tokens (16 rows) 186 / 231, 5 tokens
+// (20 rows) 342 / 232; 1 token of 34/2 heads (17 rows) 81 / 75.  Heads of 64 cross later (8/2 heads: 16 rows 37 / 66, 20 rows
+// 56 / 67), heads of 256 a little earlier (4 rows 96 / 102, 16 rows 115 / 105).
 static bool attn_narrow(long max_q, int group) { return max_q * group <= AR_ROWS; }
 static int attn_run(bool narrow, AttnParams& p, int dtype, int hd, long rows, long n_pages, cudaStream_t s) {
     const int tile = narrow ? AR_TILE : AT_TILE;
@@ -153,7 +156,11 @@ int launch_attn_paged(const void* q, long q_stride, const qmm_paged_kv* kv, cons
     p.n_seqs = seqs->n_seqs, p.total_q = seqs->total_q, p.max_kv = std::min(seqs->max_kv, ATT_MAX_KEYS);
     p.nqh = n_q_heads, p.nkv = nkv, p.group = n_q_heads / nkv, p.window = window, p.out_dtype = out_dtype;
     p.scale_log2 = kq_scale * LOG2_E;
-    // more rows whose items would not fill the GPU several times over: their tiles are shared evenly, as those of decode always are
+    // More rows: where their items would not fill the GPU several times over, their tiles are shared evenly, as those of decode
+    // always are.  The host knows the rows and not the lengths.  Measured, us whole / shared (32/8 heads of 128, f16): 912 new tokens
+    // on 8k and 16k 279 / 214, 512 on 32k 529 / 279 (shared); 100 x 60 on 1k 162 / 178, one prompt of 8000 494 / 932 (whole).  Not
+    // seen by the rule: a prompt without a past, whose items see part of the tiles that sharing counts for them (2000 tokens 51 / 99,
+    // 4000 tokens 144 / 268, shared), and one sequence far longer than the others (100 x 60 on 1k, one of them on 30k 621 / 205, whole).
     const bool narrow = attn_narrow(seqs->max_q, p.group);
     p.stream_k = ((long)p.total_q * p.group / attn_tiles_rows(hd) + 1) * nkv < 4l * sm_count();
     return attn_run(narrow, p, kv->dtype, hd, p.page_size, p.n_pages, as_stream(stream));

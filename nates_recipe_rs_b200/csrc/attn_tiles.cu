@@ -31,7 +31,9 @@ namespace qmm {
 
 constexpr int AT_TILE = 128;  // keys per tile, and rows per tile
 constexpr int AT_SEGS = 4;  // segments planned ahead
-constexpr int AT_FEW_SEQS = 64;  // up to this many sequences the planning warp finds its place alone, beyond the whole CTA does
+// Up to this many sequences (two a lane) the planning warp finds its place alone, beyond the whole CTA does: 64 x 5 tokens on 200
+// take 41 us, 65 x 5 take 47
+constexpr int AT_FEW_SEQS = 64;
 template <int HD> struct AtShape {
     static constexpr bool WIDE = HD > 128;            // one row tile, its scores in two buffers
     static constexpr int HALVES = WIDE ? 2 : 1;       // slots of a tile of keys (or values): 128 keys x up to 128 elements each
