@@ -317,7 +317,7 @@ int launch_attn_prefill_f16kv_at(const float* q, const void* k16, const void* v1
  * sequence s are rows cu_q[s] .. cu_q[s+1]-1 of the packed buffers (none, one, or many); kv_len[s] is the sequence's length with
  * them, so that row cu_q[s] + i is position kv_len[s] - (cu_q[s+1] - cu_q[s]) + i.  total_q: rows of the buffers; rows of no
  * sequence (before cu_q[0], from cu_q[n_seqs] on) are left as they were.  max_q, max_kv: at least the largest number of new
- * tokens and the largest kv_len (max_q chooses the kernel; kv_len beyond max_kv is cut to it).
+ * tokens and the largest kv_len (max_q chooses the kernel; kv_len beyond max_kv is cut to it, status 7).  n_seqs up to 2^20.
  * A pool (qmm_paged_kv, likewise): k_pages and v_pages (n_pages, page_size, n_kv_heads, head_dim) f16 or bf16, 16-byte aligned,
  * pages k_page_stride / v_page_stride elements apart (multiples of 8; 0 = back to back; the two pools may be interleaved).
  * Position t of sequence s is slot t % page_size of page page_table[s * table_stride + t / page_size]; entries past the
@@ -330,13 +330,15 @@ int launch_attn_prefill_f16kv_at(const float* q, const void* k16, const void* v1
  *   (pairs j and j + rotary_dim/2, angle position * theta^(-2j/rotary_dim), evaluated in f64); the queries go to q_out
  *   (total_q, n_q_heads * head_dim), k and v to their slots, all in the pool's type, rounded once.  q_out distinct from qkv.
  *   A token whose position is negative (kv_len smaller than the number of new tokens) has no slot: only its query is written.
+ *   Any page_size; head_dim up to 1024, a row of at most 2^22 elements.
  * launch_attn_paged: row r of q (the pool's type) against the keys of its sequence at positions up to its own:
  *   out[r,h] = sum_t w_t v_t / sum_t w_t, w_t = exp(kq_scale * q_r.k_t - max), over t <= position, and t > position - window
- *   when window > 0.  A row that sees no key is 0.  out f16, bf16 or f32.  Query head h reads kv head h / (n_q_heads /
+ *   when window > 0.  A row that sees no key is 0; an infinite value that a row does see makes that element infinite or NaN.
+ *   out f16, bf16 or f32, aligned to two elements, out_stride even, distinct from q.  Query head h reads kv head h / (n_q_heads /
  *   n_kv_heads), at most 64 per kv head; head_dim 32, 64, 96, 128 or 256; page_size a multiple of 8; kq_scale positive, at
- *   most 2.3e38 (its product with log2(e) is an f32, as kq_scale * log2(e) * q_r.k_t has to be); q 16-byte aligned, q_stride a
- *   multiple of 8; sequences of up to 2^31 - 4096 tokens (longer ones are cut to that, status 7).  A key or value that a row
- *   does not see has no influence on it, whatever it holds (NaN and infinities too).
+ *   most 2.3e38 (its product with log2(e) has to be an f32, as does q_r.k_t); q 16-byte aligned, q_stride a multiple of 8;
+ *   sequences of up to 2^31 - 4096 tokens (longer ones are cut to that, status 7).  A key or value that a row does not see has no
+ *   influence on it, whatever it holds (NaN and infinities too).
  *   scratch: qmm_attn_paged_scratch_bytes(...) bytes of caller-owned device memory, 16-byte aligned, not shared with a call that
  *   may run at the same time; nothing in it needs clearing.
  * launch_attn_packed: the same without a cache, for whole prompts: the keys and values are rows of the batch (kv_len and max_kv

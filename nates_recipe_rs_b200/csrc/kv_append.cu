@@ -2,7 +2,7 @@
 // sequences at positions of their own, of the upstream's gpu_rope_partial (gpu-core/src/infer_ops.rs:61-83,
 // gpu-core/src/kernels/f64_infer.hip:107-132: NeoX pairs (j, j + rotary_dim/2) of the first rotary_dim elements, angle
 // pos * theta^(-2j/rotary_dim)) followed by the copy into the cache.
-// Measured: 12122 tokens of 64/8 heads of 128, f32 to bf16: 122 us, 6.1 TB/s; 8 tokens 5.5 us.
+// Measured: 12122 tokens of 64/8 heads of 128, f32 to bf16: 122 us, 6.1 TB/s; 8 tokens 5.3 us.
 // One pass: a row [q | k | v] is read once, the rotated queries go to q_out and k and v to their slots, all in the cache's type
 // (one rounding from f32).  Bound by these bytes (many tokens) or by the latency of a launch (few).
 // A CTA takes a few tokens.  It finds their sequences with one parallel read of cu_q, then computes each token's sines and
