@@ -215,3 +215,26 @@ def test_workspaces_that_are_not_contiguous_are_refused(ops, ws):
     n = ops.gpu_gqa_attn_paged_scratch(b.q, b.k, b.kv_len, 8, 2, 30).numel()
     with pytest.raises(ValueError, match="scratch"):
         paged(ops, b, scratch=ws(n))
+
+
+# ---- streams ---------------------------------------------------------------------------------------------------------
+def test_calls_at_the_same_time_on_two_streams(ops):
+    """Each with a workspace of its own: decode, chunks and packed prompts side by side give what they give one after another."""
+    a = ref.Batch([1] * 20, [300 * i + 1 for i in range(20)], 32, 8, 128, 16, F16, seed=51)
+    b = ref.Batch([100, 30, 1], [3000, 700, 2000], 8, 2, 64, 16, BF16, seed=52)
+    qkv = torch.randn(900, 12 * 256, device="cuda").half()
+    c = pack(qkv, [600, 300], 8, 2, 256, F16)
+    calls = [lambda ws: paged(ops, a, scratch=ws), lambda ws: paged(ops, b, scratch=ws), lambda ws: packed(ops, c, qkv)]
+    spaces = [[ops.gpu_gqa_attn_paged_scratch(x.q, x.k, x.kv_len, x.nqh, x.max_q, x.max_kv) for x in (a, b)] + [None] for _ in range(2)]
+    want = [f(ws) for f, ws in zip(calls, spaces[0])]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(12):
+        for j, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                n = (i + j) % 3
+                got.append((n, calls[n](spaces[j][n])))
+    torch.cuda.synchronize()
+    ops.check_launch()
+    for n, out in got:
+        assert torch.equal(out, want[n])
