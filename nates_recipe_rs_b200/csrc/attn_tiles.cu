@@ -156,11 +156,6 @@ __device__ __forceinline__ void max64(const uint32_t (&s)[32], float (&m)[2]) {
 }
 // Two f32 operations at a time
 __device__ __forceinline__ uint64_t f32x2(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
